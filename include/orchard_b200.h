@@ -58,6 +58,8 @@ int orch_device_name(char* buf, size_t len);
  * table (that row's q/k/v not written); 2 an attention row's position outside the cache
  * or a bad prefill unit (its output not written); 4 an embedding id outside the vocabulary
  * (zero row); 8 a cache slot outside [0, num_slots) (no cache read or write for that row);
+ * 16 a row of orch_logits_process whose history length, bias range or mask index lies
+ * outside what the call was given (that row not written);
  * 256 a tensor-core GEMM's bounded wait ran out; 512 a peer all-reduce's wait for another
  * rank ran out. Covers the allocation-free attention entry point's flags as well. */
 int orch_device_check(uint32_t* flags_out, void* stream);
@@ -291,6 +293,71 @@ int orch_argmax_rows(const float* logits, uint32_t M, uint32_t V, int32_t* out, 
 /* Gathers fp32 residual rows x[m] = table[ids[m]] (table fp16 or fp32 [V, H]). */
 int orch_embed_rows(const int32_t* ids, const void* table, int table_dt, float* x, uint32_t M,
                     uint32_t H, uint32_t V, void* stream);
+
+/* ---- serving a batch: shared prefixes, a bounded cache, controlled logits -----------------
+ * No counterpart in the reference, which attends per sequence over a host cache that keeps
+ * every position and samples from the logits as they are (orchard/model.py:112-144,244-252). */
+/* Decode attention of rows that share long prefixes held once, beside each row's own cache
+ * entries. q, out fp16 [M, num_heads, head_dim]; head_dim 32, 64 or 128; head h reads K/V head
+ * h / (num_heads / num_kv_heads). prefix_k, prefix_v fp16 [num_prefix][num_kv_heads]
+ * [prefix_cap][head_dim]; `units` (device, 16-byte aligned) lists num_units records of four
+ * int32 (row0, rows, prefix, length): rows row0 .. row0 + rows - 1 (1..128 of them) attend to
+ * the first `length` (<= max_prefix <= prefix_cap) entries of prefix `prefix`. A row belongs to
+ * one unit at most; one in none has no prefix. Row m also attends to the first lens[m]
+ * (<= max_own <= max_seq) entries of slot slots[m] (NULL = m) of the caches, laid out
+ * [num_slots][num_kv_heads][max_seq][head_dim]; entries past that are not read. Query and
+ * entries carry their rotations, so the order of the entries does not matter. A row with
+ * nothing to attend to is zero. max_prefix and max_own bound the lengths on the device and
+ * fix how the work is cut, so a captured graph serves every length up to them.
+ * `mass` (fp32 [num_slots][num_kv_heads][max_seq], NULL = none) takes the weight that each own
+ * entry received, summed over the query heads of its K/V head: added to entries below
+ * lens[m] - 1, stored into entry lens[m] - 1 (the newest: it has no earlier weight). Rows that
+ * share a slot are taken in row order; sums have one order, so results repeat bit for bit.
+ * A row whose slot or length is out of range, or whose unit is, is not written (nor its mass)
+ * and sets device check bit 8 (slot) / 2. `workspace`, 16-byte aligned, holds
+ * orch_attention_prefix_workspace_bytes() bytes (the same arguments; track: mass given). */
+size_t orch_attention_prefix_workspace_bytes(uint32_t M, uint32_t num_heads, uint32_t num_kv_heads,
+                                             uint32_t head_dim, uint32_t num_units, uint32_t max_prefix,
+                                             uint32_t max_own, int track);
+int orch_attention_prefix(const void* q, const void* prefix_k, const void* prefix_v, const int32_t* units,
+                          uint32_t num_units, uint32_t max_prefix, uint32_t prefix_cap, uint32_t num_prefix,
+                          const void* k_cache, const void* v_cache, const int32_t* lens, const int32_t* slots,
+                          uint32_t max_own, uint32_t max_seq, uint32_t num_slots, float* mass, void* out, uint32_t M,
+                          uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim, void* workspace,
+                          size_t workspace_bytes, void* stream);
+/* Drops cache entries by accumulated weight. Each (row, K/V head) keeps n = min(lens[m], budget)
+ * of its lens[m] entries: the protected ones first (positions[e] > the row and head's largest
+ * position - recent), then by mass, equal masses by the lower index (a NaN is the smallest
+ * mass; if more than n are protected the same order picks among them). Survivors below n stay
+ * where they are; the j-th hole below n takes the j-th survivor at or above n, in K, V, mass
+ * and position. K and V ([num_slots][num_kv_heads][max_seq][head_dim] fp16) change in place;
+ * mass (fp32) and positions (int32), both [num_slots][num_kv_heads][max_seq], go to mass_out and
+ * positions_out, which are the same buffers (in place) or both others (then only entries below
+ * n of the rows' slots are written); lens_out[m] = n, in a buffer of its own. head_dim a multiple of 8;
+ * max_seq at most 1,000,000. A row whose slot or length is out of range, or whose slot an
+ * earlier row names, is left as it is and sets device check bit 8 (slot) / 2. */
+int orch_cache_evict(void* k_cache, void* v_cache, const float* mass, const int32_t* positions, const int32_t* lens,
+                     const int32_t* slots, float* mass_out, int32_t* positions_out, int32_t* lens_out, uint32_t M,
+                     uint32_t num_kv_heads, uint32_t head_dim, uint32_t max_seq, uint32_t num_slots, uint32_t budget,
+                     uint32_t recent, void* stream);
+/* Penalties, biases and grammar masks on logits [M, V] (dt ORCH_F32 or ORCH_F16, row stride ld
+ * elements; out of the same type and stride, may be logits). Column i is token id base + i (a
+ * vocabulary slice has base > 0). In fp32, in this order, per row m and token v:
+ *   history int32 [M, history_ld], its first hist_len[m] ids; penalties fp32 [M, 3] =
+ *   (repetition, presence, frequency): if v occurs in them, l = l > 0 ? l / repetition :
+ *   l * repetition; with c occurrences from index gen_start[m] on (NULL = 0),
+ *   l -= frequency * c + (c > 0 ? presence : 0). NULL history and penalties: none;
+ *   bias_ids / bias_vals [num_bias], row m's at bias_off[m] .. bias_off[m + 1] - 1 (bias_off
+ *   int32 [M + 1]): l += the bias of v, the last one if v is listed twice. NULL: none;
+ *   masks uint32 [num_masks, mask_words], row m's is mask_rows[m] (negative: none): l = -inf
+ *   unless bit v & 31 of word v >> 5 is set (ids past the words are not allowed). NULL: none.
+ * Ids outside the slice are skipped. A row whose hist_len, bias range or mask index is out of
+ * range is not written and sets device check bit 16. */
+int orch_logits_process(const void* logits, void* out, int dt, uint32_t M, uint32_t V, uint32_t ld, uint32_t base,
+                        const int32_t* history, uint32_t history_ld, const int32_t* hist_len,
+                        const int32_t* gen_start, const float* penalties, const int32_t* bias_ids,
+                        const float* bias_vals, const int32_t* bias_off, uint32_t num_bias, const uint32_t* masks,
+                        uint32_t mask_words, uint32_t num_masks, const int32_t* mask_rows, void* stream);
 
 /* ---- peer-memory all-reduce of the head split ------------------------------------------
  * The reference runs on one device (orchard/model.py:78-195 has no collective); the head

@@ -99,6 +99,13 @@ _SIGS = {
     "orch_attention_decode_noalloc": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp]),
     "orch_argmax_rows": (_i32, [_vp, _u32, _u32, _vp, _vp]),
     "orch_embed_rows": (_i32, [_vp, _vp, _i32, _vp, _u32, _u32, _u32, _vp]),
+    "orch_attention_prefix_workspace_bytes": (_sz, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _i32]),
+    "orch_attention_prefix": (_i32, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _u32, _u32, _u32,
+                                     _vp, _vp, _u32, _u32, _u32, _u32, _vp, _sz, _vp]),
+    "orch_cache_evict": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
+                                _vp]),
+    "orch_logits_process": (_i32, [_vp, _vp, _i32, _u32, _u32, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _u32,
+                                   _vp, _u32, _u32, _vp, _vp]),
     "orch_peer_region_bytes": (_sz, [_u32, _u32]),
     "orch_ipc_handle": (_i32, [_vp, _vp]),
     "orch_ipc_open": (_i32, [_vp, C.POINTER(_vp)]),

@@ -1,0 +1,665 @@
+// Attention of a batch whose rows share long prefixes, each prefix held once, beside every
+// row's own cache entries; optionally the weight each own entry received is added to a
+// running mass (the input of orch_cache_evict).
+//
+// Mathematics. Row m, head h, K/V head kv = h / G (G = num_heads / num_kv_heads):
+//   s_j = q . k_j / sqrt(hd) over the prefix keys, then the row's own entries,
+//   out = sum_j e^(s_j - max) v_j / sum_j e^(s_j - max).
+// The sums over disjoint key ranges combine: a range keeps (max, sum, weighted V), and the
+// ranges are joined by rescaling each with e^(its max - the common max).
+//
+// Work. A "unit" names consecutive rows and the prefix they share. One CTA takes a range of
+// one prefix's keys for one K/V head and a tile of the unit's query rows (rows x G heads of
+// that K/V head), so the prefix is read once for all of them; another CTA takes a range of
+// one row's own entries for its G heads. Both run the same tensor-core tile: S = Q K^T in
+// m16n8k16 MMAs (exact products of fp16 values, fp32 sums), an online softmax in fp32, O += P V
+// with P rounded to fp16. That rounding costs 2^-12 relative per weight, below the rounding of
+// the fp16 output; P is scaled by 2^10 so that weights down to 2^-24 of the largest stay
+// normal numbers. The sums l take the unrounded weights.
+//
+// Layout of a CTA: 4 warps. A tile of 64 rows gives each warp 16 rows and all 64 keys of a
+// block; a tile of 16 or 32 rows splits the block's keys over 4 or 2 warps instead, whose
+// (max, sum, O) meet in shared memory at the end, so few rows still keep every warp at work.
+// K and V blocks of 64 keys are copied by cp.async into a double buffer.
+#include <algorithm>
+
+#include "orch_common.cuh"
+
+namespace orch {
+
+namespace {
+
+constexpr int kApKeys = 64;         // keys per block
+constexpr int kApMaxUnitRows = 128;  // rows of a unit
+constexpr uint32_t kApMaxLen = 1u << 29;  // entries of a slot: twice that stays an int
+constexpr float kApShift = 10.f;    // P is held as 2^10 e^(s - max)
+
+struct ApArgs {
+  const __half* q;
+  const __half* kp;
+  const __half* vp;
+  const int4* units;  // (row0, rows, prefix slot, prefix length)
+  int num_units, max_prefix, prefix_cap, num_prefix;
+  const __half* kc;
+  const __half* vc;
+  const int* lens;
+  const int* slots;
+  int max_own, max_seq, num_slots;
+  float* mass;
+  __half* out;
+  int M, nh, nkv, G;
+  int wr_p, wr_o;        // warps along the rows of a prefix tile / an own tile
+  int tiles_p, tiles_o;  // row tiles per unit / per row
+  int S_p, S_o;          // key ranges of a prefix / of a row's own entries
+  int blocks_p;          // CTAs of the prefix part (the first ones of the grid)
+  int direct;            // one range in all: the output is written by the attention kernel
+  float* acc;            // [M * nh][S][HD]
+  float2* stat;          // [M * nh][S]: (max, sum), in powers of two
+  float* scores;         // [M * nh][lds], with mass only
+  int lds;
+  uint32_t* check;
+};
+
+__device__ __forceinline__ void ap_cp16(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src), "r"(ok ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void ap_ldsm4(const __half* p, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+}
+__device__ __forceinline__ void ap_ldsm4_t(const __half* p, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
+}
+__device__ __forceinline__ float ap_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Keys of range s of n keys cut into at most S ranges of whole blocks.
+__host__ __device__ __forceinline__ int ap_range(int n, int S) {
+  const int per = (n + S - 1) / S;
+  return (per + kApKeys - 1) / kApKeys * kApKeys;
+}
+
+// A unit that names rows, a prefix slot and a length inside what the call was given.
+__device__ __forceinline__ bool ap_unit_ok(const ApArgs& a, const int4& u) {
+  return u.y >= 1 && u.y <= kApMaxUnitRows && u.x >= 0 && u.x < a.M && u.y <= a.M - u.x && u.w >= 0 &&
+         u.w <= a.max_prefix && u.z >= 0 && u.z < a.num_prefix;
+}
+// The row's cache slot and own length, or false when either lies outside the cache.
+__device__ __forceinline__ bool ap_row(const ApArgs& a, int m, int& slot, int& len) {
+  slot = a.slots ? a.slots[m] : m;
+  len = a.lens[m];
+  return slot >= 0 && slot < a.num_slots && len >= 0 && len <= a.max_own;
+}
+
+// One tile: query rows i0 .. i0 + n - 1 of the (row, head of kv) pairs starting at row m0,
+// keys [j0, j1) of K/V rows at kb / vb; partials go to range `split`.
+template <int HD, int WR>
+__device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, int kv, const __half* kb,
+                                        const __half* vb, int j0, int j1, int split, float* srow) {
+  constexpr int WK = 4 / WR, TR = 16 * WR, P = HD + 8, TILE = kApKeys * P, KT = kApKeys / 8 / WK;
+  extern __shared__ __align__(16) uint8_t ap_smem[];
+  __half* buf = reinterpret_cast<__half*>(ap_smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int wrow = warp % WR, wkey = warp / WR;
+  const int nb = (j1 - j0 + kApKeys - 1) / kApKeys;
+
+  auto issue = [&](int b) {
+    __half* kd = buf + (b & 1) * 2 * TILE;
+    __half* vd = kd + TILE;
+    constexpr int CPR = HD / 8;  // 16-byte pieces per row
+#pragma unroll
+    for (int j = 0; j < kApKeys * CPR / 128; ++j) {
+      const int i = tid + 128 * j, r = i / CPR, d8 = (i % CPR) * 8, key = j0 + b * kApKeys + r;
+      const bool ok = key < j1;
+      const size_t off = ok ? (size_t)key * HD + d8 : 0;
+      ap_cp16(kd + r * P + d8, kb + off, ok);
+      ap_cp16(vd + r * P + d8, vb + off, ok);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  issue(0);
+
+  // Q rows through buffer 1, then into registers as A fragments
+  __half* qs = buf + 2 * TILE;
+  for (int i = tid; i < TR * (HD / 8); i += 128) {
+    const int r = i / (HD / 8), d8 = (i % (HD / 8)) * 8;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (r < n) {
+      const int m = m0 + (i0 + r) / a.G, h = kv * a.G + (i0 + r) % a.G;
+      v = *reinterpret_cast<const uint4*>(a.q + ((size_t)m * a.nh + h) * HD + d8);
+    }
+    *reinterpret_cast<uint4*>(qs + r * P + d8) = v;
+  }
+  __syncthreads();
+  const int qr = wrow * 16 + g;  // this thread's rows: qr and qr + 8
+  uint32_t qa[HD / 16][4];
+#pragma unroll
+  for (int kk = 0; kk < HD / 16; ++kk) {
+    qa[kk][0] = *reinterpret_cast<const uint32_t*>(qs + qr * P + 16 * kk + 2 * c);
+    qa[kk][1] = *reinterpret_cast<const uint32_t*>(qs + (qr + 8) * P + 16 * kk + 2 * c);
+    qa[kk][2] = *reinterpret_cast<const uint32_t*>(qs + qr * P + 16 * kk + 8 + 2 * c);
+    qa[kk][3] = *reinterpret_cast<const uint32_t*>(qs + (qr + 8) * P + 16 * kk + 8 + 2 * c);
+  }
+  __syncthreads();  // buffer 1 is free for block 1
+
+  float o[HD / 8][4];
+#pragma unroll
+  for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+  float m0r = -INFINITY, m1r = -INFINITY, l0 = 0.f, l1 = 0.f;
+  const float scale = rsqrtf((float)HD) * 1.4426950408889634f;  // scores in powers of two
+  const int lm = lane >> 3, lr = lane & 7;
+
+  for (int b = 0; b < nb; ++b) {
+    if (b + 1 < nb) {
+      issue(b + 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncthreads();
+    const __half* ks = buf + (b & 1) * 2 * TILE;
+    const __half* vs = ks + TILE;
+    const int kt0 = wkey * KT;  // first 8-key tile of this warp
+
+    float sc[KT][4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; kk += 2) {
+        uint32_t bb[4];
+        ap_ldsm4(ks + (8 * (kt0 + t) + lr) * P + 16 * kk + 8 * lm, bb);
+        mma_16816(sc[t], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bb[0], bb[1]);
+        mma_16816(sc[t], qa[kk + 1][0], qa[kk + 1][1], qa[kk + 1][2], qa[kk + 1][3], bb[2], bb[3]);
+      }
+    }
+    float bm0 = -INFINITY, bm1 = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool ok = j0 + b * kApKeys + 8 * (kt0 + t) + 2 * c + e < j1;
+        sc[t][e] = ok ? sc[t][e] * scale : -INFINITY;
+        sc[t][2 + e] = ok ? sc[t][2 + e] * scale : -INFINITY;
+        bm0 = fmaxf(bm0, sc[t][e]);
+        bm1 = fmaxf(bm1, sc[t][2 + e]);
+      }
+    if (srow != nullptr) {  // the own entries' scores, for their weights (rows are the G heads)
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int key = j0 + b * kApKeys + 8 * (kt0 + t) + 2 * c + e;
+          if (key < j1) {
+            if (qr < n) srow[(size_t)(i0 + qr) * a.lds + key] = sc[t][e];
+            if (qr + 8 < n) srow[(size_t)(i0 + qr + 8) * a.lds + key] = sc[t][2 + e];
+          }
+        }
+    }
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+      bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, x));
+      bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, x));
+    }
+    // a warp's keys may all lie past j1: its maximum is then still -inf and stands for 0
+    const float mn0 = fmaxf(m0r, bm0), mn1 = fmaxf(m1r, bm1);
+    const float r0 = mn0 == -INFINITY ? 0.f : mn0 - kApShift, r1 = mn1 == -INFINITY ? 0.f : mn1 - kApShift;
+    const float al0 = ap_exp2(m0r - (mn0 == -INFINITY ? 0.f : mn0)), al1 = ap_exp2(m1r - (mn1 == -INFINITY ? 0.f : mn1));
+    m0r = mn0;
+    m1r = mn1;
+    float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      sc[t][0] = ap_exp2(sc[t][0] - r0);
+      sc[t][1] = ap_exp2(sc[t][1] - r0);
+      sc[t][2] = ap_exp2(sc[t][2] - r1);
+      sc[t][3] = ap_exp2(sc[t][3] - r1);
+      rs0 += sc[t][0] + sc[t][1];
+      rs1 += sc[t][2] + sc[t][3];
+    }
+    l0 = l0 * al0 + rs0;
+    l1 = l1 * al1 + rs1;
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d) {
+      o[d][0] *= al0;
+      o[d][1] *= al0;
+      o[d][2] *= al1;
+      o[d][3] *= al1;
+    }
+#pragma unroll
+    for (int j = 0; j < KT / 2; ++j) {
+      uint32_t pa[4];
+      pa[0] = h2_bits(__floats2half2_rn(sc[2 * j][0], sc[2 * j][1]));
+      pa[1] = h2_bits(__floats2half2_rn(sc[2 * j][2], sc[2 * j][3]));
+      pa[2] = h2_bits(__floats2half2_rn(sc[2 * j + 1][0], sc[2 * j + 1][1]));
+      pa[3] = h2_bits(__floats2half2_rn(sc[2 * j + 1][2], sc[2 * j + 1][3]));
+#pragma unroll
+      for (int d = 0; d < HD / 8; d += 2) {
+        uint32_t bb[4];
+        ap_ldsm4_t(vs + (8 * kt0 + 16 * j + 8 * (lm & 1) + lr) * P + 8 * d + 8 * (lm >> 1), bb);
+        mma_16816(o[d], pa[0], pa[1], pa[2], pa[3], bb[0], bb[1]);
+        mma_16816(o[d + 1], pa[0], pa[1], pa[2], pa[3], bb[2], bb[3]);
+      }
+    }
+    __syncthreads();  // buffer b & 1 is free for block b + 2
+  }
+#pragma unroll
+  for (int x = 1; x <= 2; x <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+  }
+
+  // the tile's rows in shared memory: warp wkey's part of O [row][HD] and (max, sum) per row
+  constexpr int OP = HD + 4;
+  float* os = reinterpret_cast<float*>(ap_smem);        // [WK][TR][OP]
+  float2* ss = reinterpret_cast<float2*>(os + WK * TR * OP);  // [WK][TR]
+  {
+    float* w = os + (size_t)(wkey * TR + qr) * OP + 2 * c;
+#pragma unroll
+    for (int d = 0; d < HD / 8; ++d) {
+      *reinterpret_cast<float2*>(w + 8 * d) = make_float2(o[d][0], o[d][1]);
+      *reinterpret_cast<float2*>(w + 8 * OP + 8 * d) = make_float2(o[d][2], o[d][3]);
+    }
+    if (c == 0) {
+      ss[wkey * TR + qr] = make_float2(m0r, l0);
+      ss[wkey * TR + qr + 8] = make_float2(m1r, l1);
+    }
+  }
+  __syncthreads();
+  constexpr int LPR = HD / 4;  // threads per row, four values each
+  const int S = a.S_p + a.S_o;
+  for (int i = tid; i < n * LPR; i += 128) {
+    const int r = i / LPR, d = (i % LPR) * 4;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) mx = fmaxf(mx, ss[w * TR + r].x);
+    float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float2 st = ss[w * TR + r];
+      const float f = st.x == -INFINITY ? 0.f : ap_exp2(st.x - mx);
+      const float4 ov = *reinterpret_cast<const float4*>(os + (size_t)(w * TR + r) * OP + d);
+      l = fmaf(f, st.y, l);
+      v[0] = fmaf(f, ov.x, v[0]);
+      v[1] = fmaf(f, ov.y, v[1]);
+      v[2] = fmaf(f, ov.z, v[2]);
+      v[3] = fmaf(f, ov.w, v[3]);
+    }
+    const size_t mh = (size_t)(m0 + (i0 + r) / a.G) * a.nh + kv * a.G + (i0 + r) % a.G;
+    if (a.direct) {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      uint2 h;
+      h.x = h2_bits(__floats2half2_rn(v[0] * inv, v[1] * inv));
+      h.y = h2_bits(__floats2half2_rn(v[2] * inv, v[3] * inv));
+      *reinterpret_cast<uint2*>(a.out + mh * HD + d) = h;
+    } else {
+      *reinterpret_cast<float4*>(a.acc + (mh * S + split) * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+      if (d == 0) a.stat[mh * S + split] = make_float2(mx, l);
+    }
+  }
+}
+
+template <int HD>
+__device__ __forceinline__ void ap_tile_wr(int wr, const ApArgs& a, int m0, int i0, int n, int kv, const __half* kb,
+                                           const __half* vb, int j0, int j1, int split, float* srow) {
+  if (wr == 1)
+    ap_tile<HD, 1>(a, m0, i0, n, kv, kb, vb, j0, j1, split, srow);
+  else if (wr == 2)
+    ap_tile<HD, 2>(a, m0, i0, n, kv, kb, vb, j0, j1, split, srow);
+  else
+    ap_tile<HD, 4>(a, m0, i0, n, kv, kb, vb, j0, j1, split, srow);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  int b = blockIdx.x;
+  if (b < a.blocks_p) {  // a range of a prefix for a tile of the unit's query rows
+    // row tiles fastest: the tiles that read the same keys run together
+    const int tile = b % a.tiles_p;
+    b /= a.tiles_p;
+    const int split = b % a.S_p;
+    b /= a.S_p;
+    const int kv = b % a.nkv;
+    const int4 u = a.units[b / a.nkv];
+    if (!ap_unit_ok(a, u)) {
+      if (threadIdx.x == 0) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
+      return;
+    }
+    const int tr = 16 * a.wr_p, i0 = tile * tr, n = min(tr, u.y * a.G - i0);
+    const int per = ap_range(u.w, a.S_p), j0 = split * per, j1 = min(u.w, j0 + per);
+    if (n <= 0 || j0 >= j1) return;
+    const size_t base = ((size_t)u.z * a.nkv + kv) * a.prefix_cap * HD;
+    ap_tile_wr<HD>(a.wr_p, a, u.x, i0, n, kv, a.kp + base, a.vp + base, j0, j1, split, nullptr);
+    return;
+  }
+  b -= a.blocks_p;  // a range of one row's own entries for the G heads of a K/V head
+  const int tile = b % a.tiles_o;
+  b /= a.tiles_o;
+  const int split = b % a.S_o;
+  b /= a.S_o;
+  const int kv = b % a.nkv, m = b / a.nkv;
+  int slot, len;
+  if (!ap_row(a, m, slot, len)) {
+    if (threadIdx.x == 0) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
+    return;
+  }
+  const int tr = 16 * a.wr_o, i0 = tile * tr, n = min(tr, a.G - i0);
+  const int per = ap_range(len, a.S_o), j0 = split * per, j1 = min(len, j0 + per);
+  if (j0 >= j1) {
+    if (a.direct && len == 0) {  // nothing to attend to
+      for (int i = threadIdx.x; i < n * HD; i += 128)
+        a.out[((size_t)m * a.nh + kv * a.G + i0) * HD + i] = __float2half_rn(0.f);
+    }
+    return;
+  }
+  const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
+  float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
+  ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, a.kc + base, a.vc + base, j0, j1, a.S_p + split, srow);
+}
+
+// Ranges of row m that hold keys: prefix ranges 0 .. np - 1, own ranges S_p .. S_p + no - 1.
+// False when the row or its unit was rejected. (Called by whole warps.)
+__device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int& len, int& np, int& no) {
+  if (!ap_row(a, m, slot, len)) return false;
+  const int lane = threadIdx.x & 31;
+  int plen = 0, bad = 0;
+  for (int u0 = 0; u0 < a.num_units; u0 += 32) {
+    const int i = u0 + lane;
+    if (i < a.num_units) {
+      const int4 u = a.units[i];
+      if (m >= u.x && (long long)m < (long long)u.x + u.y) {
+        if (ap_unit_ok(a, u))
+          plen = max(plen, u.w);
+        else
+          bad = 1;
+      }
+    }
+  }
+  plen = __reduce_max_sync(0xffffffffu, plen);
+  if (__any_sync(0xffffffffu, bad)) return false;
+  np = plen > 0 ? (plen + ap_range(plen, a.S_p) - 1) / ap_range(plen, a.S_p) : 0;
+  no = len > 0 ? (len + ap_range(len, a.S_o) - 1) / ap_range(len, a.S_o) : 0;
+  return true;
+}
+
+// The common maximum and sum of row-head mh over its ranges. (Called by whole warps.)
+__device__ __forceinline__ float2 ap_total(const ApArgs& a, size_t mh, int np, int no) {
+  const int lane = threadIdx.x & 31;
+  const float2* st = a.stat + mh * (a.S_p + a.S_o);
+  float mx = -INFINITY;
+  for (int s = lane; s < np + no; s += 32) mx = fmaxf(mx, st[s < np ? s : a.S_p + s - np].x);
+  mx = warp_max(mx);
+  float l = 0.f;
+  for (int s = lane; s < np + no; s += 32) {
+    const float2 v = st[s < np ? s : a.S_p + s - np];
+    l += v.x == -INFINITY ? v.y : ap_exp2(v.x - mx) * v.y;
+  }
+  return make_float2(mx, warp_sum(l));
+}
+
+// Joins the ranges: one warp per (row, head) for the output; with mass, further CTAs each
+// take kMassEntries entries of one (row, K/V head).
+constexpr int kMassEntries = 1024;
+
+template <int HD>
+__global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, int blocks_out, int chunks) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int S = a.S_p + a.S_o;
+  if (blockIdx.x < blocks_out) {
+    const int mh = blockIdx.x * 4 + warp;
+    if (mh >= a.M * a.nh) return;
+    int slot, len, np, no;
+    if (!ap_ranges(a, mh / a.nh, slot, len, np, no)) return;
+    const float2 tot = ap_total(a, mh, np, no);
+    constexpr int V = HD / 32;  // values per lane
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+    const float* ac = a.acc + (size_t)mh * S * HD + lane * V;
+    const float2* st = a.stat + (size_t)mh * S;
+    const int n = np + no;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const int r = s < np ? s : a.S_p + s - np;
+      const float m = st[r].x, f = m == -INFINITY ? 0.f : ap_exp2(m - tot.x);
+      if (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(ac + (size_t)r * HD);
+        v[0] = fmaf(f, x.x, v[0]);
+        v[1 % V] = fmaf(f, x.y, v[1 % V]);
+        v[2 % V] = fmaf(f, x.z, v[2 % V]);
+        v[3 % V] = fmaf(f, x.w, v[3 % V]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fmaf(f, ac[(size_t)r * HD + i], v[i]);
+      }
+    }
+    const float inv = tot.y == 0.f ? 0.f : 1.0f / tot.y;  // nothing to attend to: zeros
+    __half* op = a.out + (size_t)mh * HD + lane * V;
+    if (V == 4) {
+      uint2 h;
+      h.x = h2_bits(__floats2half2_rn(v[0] * inv, v[1 % V] * inv));
+      h.y = h2_bits(__floats2half2_rn(v[2 % V] * inv, v[3 % V] * inv));
+      *reinterpret_cast<uint2*>(op) = h;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) op[i] = __float2half_rn(v[i] * inv);
+    }
+    return;
+  }
+  // Weights of the own entries. The first of the rows that share a slot takes them all, in row
+  // order, so the sums have one order.
+  int b = blockIdx.x - blocks_out;
+  const int chunk = b % chunks;
+  b /= chunks;
+  const int kv = b % a.nkv, m = b / a.nkv;
+  int slot, len, np, no;
+  if (!ap_ranges(a, m, slot, len, np, no)) return;
+  __shared__ int any;
+  if (threadIdx.x == 0) any = 0;
+  __syncthreads();
+  int mine = 0;  // whether another row of the call has this slot: 1 an earlier one, 2 a later one
+  for (int r = threadIdx.x; r < a.M; r += 128)
+    if (r != m && (a.slots ? a.slots[r] : r) == slot) mine |= r < m ? 1 : 2;
+  if (mine) atomicOr(&any, mine);
+  __syncthreads();
+  // an earlier row of the slot that was itself rejected takes nothing: look for a valid one
+  if (any & 1) {
+    for (int r = 0; r < m; ++r) {
+      if ((a.slots ? a.slots[r] : r) != slot) continue;
+      int s2, l2, p2, o2;
+      if (ap_ranges(a, r, s2, l2, p2, o2)) return;
+    }
+  }
+  float* mass = a.mass + ((size_t)slot * a.nkv + kv) * a.max_seq;
+  const int last = (any & 2) ? a.M - 1 : m;
+  for (int r = m; r <= last; ++r) {
+    if ((a.slots ? a.slots[r] : r) != slot) continue;
+    int s2;
+    if (r != m && !ap_ranges(a, r, s2, len, np, no)) continue;
+    const int e0 = chunk * kMassEntries;
+    if (e0 >= len) continue;
+    float w[kMassEntries / 128];
+#pragma unroll
+    for (int i = 0; i < kMassEntries / 128; ++i) w[i] = 0.f;
+    for (int h = kv * a.G; h < (kv + 1) * a.G; ++h) {
+      const size_t mh = (size_t)r * a.nh + h;
+      const float2 tot = ap_total(a, mh, np, no);
+      const float ref = tot.x == -INFINITY ? 0.f : tot.x - kApShift, inv = tot.y == 0.f ? 0.f : 1.0f / tot.y;
+      const float* sr = a.scores + mh * a.lds;
+#pragma unroll
+      for (int i = 0; i < kMassEntries / 128; ++i) {
+        const int e = e0 + threadIdx.x + 128 * i;
+        if (e < len) w[i] = fmaf(ap_exp2(sr[e] - ref), inv, w[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kMassEntries / 128; ++i) {
+      const int e = e0 + threadIdx.x + 128 * i;
+      if (e < len) mass[e] = e == len - 1 ? w[i] : mass[e] + w[i];
+    }
+  }
+}
+
+// How a call is cut: rows per tile, key ranges, workspace. The same for the size query.
+struct ApPlan {
+  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, direct, lds;
+  size_t acc_floats, stat_floats, score_floats;
+  size_t bytes() const { return (acc_floats + stat_floats + score_floats) * sizeof(float); }
+};
+
+int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_units, uint32_t max_prefix,
+               uint32_t max_own, int track) {
+  ApPlan p;
+  p.G = (int)(nh / nkv);
+  const int rows_p = (int)std::min<uint32_t>(M, kApMaxUnitRows) * p.G;
+  p.wr_p = ap_wr(rows_p);
+  p.wr_o = ap_wr(p.G);
+  p.tiles_p = (rows_p + 16 * p.wr_p - 1) / (16 * p.wr_p);
+  p.tiles_o = (p.G + 16 * p.wr_o - 1) / (16 * p.wr_o);
+  const int want = 6 * num_sms();  // two rounds of three CTAs per SM
+  const auto ranges = [&](size_t ctas, uint32_t keys, int least) {
+    const size_t s = (want + ctas - 1) / std::max<size_t>(ctas, 1);
+    return (int)std::max<size_t>(1, std::min<size_t>(s, (keys + least - 1) / least));
+  };
+  p.S_p = num_units && max_prefix ? ranges((size_t)num_units * nkv * p.tiles_p, max_prefix, 64 * p.wr_p + 64) : 0;
+  p.S_o = ranges((size_t)M * nkv * p.tiles_o, max_own, 64);  // at least one: rows are checked there
+  p.direct = p.S_p == 0 && p.S_o == 1 && !track;
+  const size_t mh = (size_t)M * nh, S = p.S_p + p.S_o;
+  p.acc_floats = p.direct ? 0 : mh * S * hd;
+  p.stat_floats = p.direct ? 0 : (mh * S * 2 + 3) / 4 * 4;
+  p.lds = (int)((max_own + 3) / 4 * 4);
+  p.score_floats = track ? mh * p.lds : 0;
+  return p;
+}
+
+template <int HD>
+int ap_launch(const ApArgs& a, cudaStream_t st) {
+  constexpr int kSmem = 4 * kApKeys * (HD + 8) * 2;
+  constexpr int kJoin = 64 * (HD + 4) * 4 + 64 * 8;  // WK x TR = 64 rows of O and their statistics
+  constexpr int smem = kSmem > kJoin ? kSmem : kJoin;
+  static bool attr_done[64] = {};
+  const int dev = device_index();
+  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr_done[dev] = true;
+  }
+  const dim3 none(0, 0, 0);
+  const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
+  if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
+  if (blocks > 0)
+    ORCH_CUDA(launch_k_serial(attn_prefix_kernel<HD>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
+  if (!a.direct) {
+    const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
+    const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
+    const size_t jb = (size_t)blocks_out + (size_t)a.M * a.nkv * chunks;
+    if (jb > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
+    ORCH_CUDA(launch_k(attn_prefix_join_kernel<HD>, dim3((unsigned)jb), dim3(128), 0, st, none, a, blocks_out,
+                       std::max(chunks, 1)));
+  }
+  return check_launch("attention_prefix");
+}
+
+bool ap_shape_ok(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd) {
+  return nh > 0 && nkv > 0 && nh % nkv == 0 && nh <= 65535 && (hd == 32 || hd == 64 || hd == 128) &&
+         (uint64_t)M * nh <= 0x7fffffffu;
+}
+
+}  // namespace
+
+}  // namespace orch
+
+using namespace orch;
+
+extern "C" size_t orch_attention_prefix_workspace_bytes(uint32_t M, uint32_t num_heads, uint32_t num_kv_heads,
+                                                        uint32_t head_dim, uint32_t num_units, uint32_t max_prefix,
+                                                        uint32_t max_own, int track) {
+  if (M == 0 || !ap_shape_ok(M, num_heads, num_kv_heads, head_dim)) return 0;
+  return ap_plan(M, num_heads, num_kv_heads, head_dim, num_units, max_prefix, max_own, track).bytes();
+}
+
+// No counterpart in the reference, which attends per sequence over a host cache
+// (orchard/model.py:112-144): the rows there share no keys and keep every position.
+extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const void* prefix_v, const int32_t* units,
+                                     uint32_t num_units, uint32_t max_prefix, uint32_t prefix_cap, uint32_t num_prefix,
+                                     const void* k_cache, const void* v_cache, const int32_t* lens,
+                                     const int32_t* slots, uint32_t max_own, uint32_t max_seq, uint32_t num_slots,
+                                     float* mass, void* out, uint32_t M, uint32_t num_heads, uint32_t num_kv_heads,
+                                     uint32_t head_dim, void* workspace, size_t workspace_bytes, void* stream) {
+  if (M == 0) return ORCH_OK;
+  ORCH_REQUIRE(q && k_cache && v_cache && lens && out, "attention_prefix: null pointer");
+  ORCH_REQUIRE(num_units == 0 || max_prefix == 0 || (prefix_k && prefix_v && units), "attention_prefix: null prefix");
+  ORCH_REQUIRE(num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0,
+               "attention_prefix: num_heads must be a multiple of num_kv_heads");
+  ORCH_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128, "attention_prefix: head_dim must be 32, 64 or 128");
+  ORCH_REQUIRE(max_seq > 0 && max_seq <= kApMaxLen && num_slots > 0 && num_slots <= 0x7fffffffu && max_own <= max_seq,
+               "attention_prefix: bad cache shape (max_own must not exceed max_seq)");
+  ORCH_REQUIRE(num_units == 0 || max_prefix == 0 ||
+                   (max_prefix <= prefix_cap && prefix_cap <= kApMaxLen && num_prefix > 0 && num_prefix <= 0x7fffffffu &&
+                    num_units <= 0x7fffffffu),
+               "attention_prefix: bad prefix shape (max_prefix must not exceed prefix_cap)");
+  ORCH_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)prefix_k |
+                 (uintptr_t)prefix_v | (uintptr_t)units | (uintptr_t)workspace) & 15) == 0,
+               "attention_prefix: buffers must be 16-byte aligned");
+  if (!ap_shape_ok(M, num_heads, num_kv_heads, head_dim))
+    return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads");
+  const ApPlan p = ap_plan(M, num_heads, num_kv_heads, head_dim, num_units, max_prefix, max_own, mass != nullptr);
+  ORCH_REQUIRE(workspace_bytes >= p.bytes() && (p.bytes() == 0 || workspace != nullptr),
+               "attention_prefix: workspace too small");
+  ApArgs a;
+  a.q = static_cast<const __half*>(q);
+  a.kp = static_cast<const __half*>(prefix_k);
+  a.vp = static_cast<const __half*>(prefix_v);
+  a.units = reinterpret_cast<const int4*>(units);
+  a.num_units = p.S_p ? (int)num_units : 0;
+  a.max_prefix = (int)max_prefix;
+  a.prefix_cap = (int)prefix_cap;
+  a.num_prefix = (int)num_prefix;
+  a.kc = static_cast<const __half*>(k_cache);
+  a.vc = static_cast<const __half*>(v_cache);
+  a.lens = lens;
+  a.slots = slots;
+  a.max_own = (int)max_own;
+  a.max_seq = (int)max_seq;
+  a.num_slots = (int)num_slots;
+  a.mass = mass;
+  a.out = static_cast<__half*>(out);
+  a.M = (int)M;
+  a.nh = (int)num_heads;
+  a.nkv = (int)num_kv_heads;
+  a.G = p.G;
+  a.wr_p = p.wr_p;
+  a.wr_o = p.wr_o;
+  a.tiles_p = p.tiles_p;
+  a.tiles_o = p.tiles_o;
+  a.S_p = p.S_p;
+  a.S_o = p.S_o;
+  const uint64_t blocks_p = (uint64_t)a.num_units * num_kv_heads * p.tiles_p * p.S_p;
+  if (blocks_p > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many units for one launch");
+  a.blocks_p = (int)blocks_p;
+  a.direct = p.direct;
+  a.acc = static_cast<float*>(workspace);
+  a.stat = reinterpret_cast<float2*>(a.acc + p.acc_floats);
+  a.scores = a.acc + p.acc_floats + p.stat_floats;
+  a.lds = p.lds;
+  ORCH_CHECK_WORD(a.check);
+  cudaStream_t st = as_stream(stream);
+  switch (head_dim) {
+    case 32: return ap_launch<32>(a, st);
+    case 64: return ap_launch<64>(a, st);
+    default: return ap_launch<128>(a, st);
+  }
+}
