@@ -148,14 +148,19 @@ def last_error() -> str:
     return (lib().orch_last_error() or b"").decode(errors="replace")
 
 
+_fns = {}  # name -> typed entry point, filled at its first call
+
+
 def call(name: str, *args) -> int:
     """Calls an int-returning entry point, raising OrchardError on a nonzero status.
 
     Tensor arguments are passed by device address and stay referenced for the duration of
     the call; work enqueued on a stream is ordered before any later reuse of their memory
     by the caching allocator on that stream."""
-    args = tuple(a.data_ptr() if hasattr(a, "data_ptr") else a for a in args)
-    rc = getattr(lib(), name)(*args)
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(lib(), name)
+    rc = f(*[a if a is None or a.__class__ is int or not hasattr(a, "data_ptr") else a.data_ptr() for a in args])
     if rc != 0:
         raise OrchardError(name, rc, last_error())
     return rc

@@ -370,7 +370,6 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
 // Ranges of row m that hold keys: prefix ranges 0 .. np - 1, own ranges S_p .. S_p + no - 1.
 // False when the row or its unit was rejected. (Called by whole warps.)
 __device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int& len, int& np, int& no) {
-  if (!ap_row(a, m, slot, len)) return false;
   const int lane = threadIdx.x & 31;
   int plen = 0, bad = 0;
   for (int u0 = 0; u0 < a.num_units; u0 += 32) {
@@ -385,12 +384,18 @@ __device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int
       }
     }
   }
+  const bool ok = ap_row(a, m, slot, len);
   plen = __reduce_max_sync(0xffffffffu, plen);
-  if (__any_sync(0xffffffffu, bad)) return false;
+  if (__any_sync(0xffffffffu, bad) || !ok) return false;
   np = plen > 0 ? (plen + ap_range(plen, a.S_p) - 1) / ap_range(plen, a.S_p) : 0;
   no = len > 0 ? (len + ap_range(len, a.S_o) - 1) / ap_range(len, a.S_o) : 0;
   return true;
 }
+
+template <int V>
+struct alignas(4 * V) ApVec {
+  float v[V];
+};
 
 // The common maximum and sum of row-head mh over its ranges. (Called by whole warps.)
 __device__ __forceinline__ float2 ap_total(const ApArgs& a, size_t mh, int np, int no) {
@@ -420,31 +425,51 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
   if (blockIdx.x < blocks_out) {
     const int mh = blockIdx.x * 4 + warp;
     if (mh >= a.M * a.nh) return;
+    // The first ranges' records are requested before it is known which of them hold keys, so
+    // that the kernel waits on L2 once; what a range without keys left there is not used.
+    constexpr int V = HD / 32, U = 8;  // values per lane, ranges requested ahead
+    const float* ac = a.acc + (size_t)mh * S * HD + lane * V;
+    const float2* st = a.stat + (size_t)mh * S;
+    ApVec<V> pre[U];
+#pragma unroll
+    for (int s = 0; s < U; ++s)
+      if (s < S) pre[s] = *reinterpret_cast<const ApVec<V>*>(ac + (size_t)s * HD);
+    float2 sl = lane < S ? st[lane] : make_float2(0.f, 0.f);
     int slot, len, np, no;
     if (!ap_ranges(a, mh / a.nh, slot, len, np, no)) return;
-    const float2 tot = ap_total(a, mh, np, no);
-    constexpr int V = HD / 32;  // values per lane
+    auto live = [&](int s) { return s < np || (s >= a.S_p && s < a.S_p + no); };
+    if (!live(lane)) sl = make_float2(-INFINITY, 0.f);
+    float mx = sl.x;
+    for (int s = lane + 32; s < S; s += 32)
+      if (live(s)) mx = fmaxf(mx, st[s].x);
+    mx = warp_max(mx);
+    auto weight = [&](float m) { return m == -INFINITY ? 0.f : ap_exp2(m - mx); };
+    const float wl = weight(sl.x);
+    // a range whose maximum is -inf has sum 0, or NaN where a key was NaN: that one is kept
+    float l = sl.x == -INFINITY ? sl.y : wl * sl.y;
+    for (int s = lane + 32; s < S; s += 32)
+      if (live(s)) l += st[s].x == -INFINITY ? st[s].y : weight(st[s].x) * st[s].y;
+    l = warp_sum(l);
     float v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = 0.f;
-    const float* ac = a.acc + (size_t)mh * S * HD + lane * V;
-    const float2* st = a.stat + (size_t)mh * S;
-    const int n = np + no;
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const int r = s < np ? s : a.S_p + s - np;
-      const float m = st[r].x, f = m == -INFINITY ? 0.f : ap_exp2(m - tot.x);
-      if (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(ac + (size_t)r * HD);
-        v[0] = fmaf(f, x.x, v[0]);
-        v[1 % V] = fmaf(f, x.y, v[1 % V]);
-        v[2 % V] = fmaf(f, x.z, v[2 % V]);
-        v[3 % V] = fmaf(f, x.w, v[3 % V]);
-      } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = fmaf(f, ac[(size_t)r * HD + i], v[i]);
+    for (int s = 0; s < U; ++s) {
+      const float f = __shfl_sync(0xffffffffu, wl, s);
+      if (live(s))
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fmaf(f, pre[s].v[i], v[i]);
+    }
+#pragma unroll 4
+    for (int s = U; s < S; ++s) {
+      const float f = s < 32 ? __shfl_sync(0xffffffffu, wl, s & 31) : live(s) ? weight(st[s].x) : 0.f;
+      if (live(s)) {
+        const ApVec<V> x = *reinterpret_cast<const ApVec<V>*>(ac + (size_t)s * HD);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = fmaf(f, x.v[i], v[i]);
       }
     }
+    const float2 tot = make_float2(mx, l);
     const float inv = tot.y == 0.f ? 0.f : 1.0f / tot.y;  // nothing to attend to: zeros
     __half* op = a.out + (size_t)mh * HD + lane * V;
     if (V == 4) {

@@ -9,8 +9,11 @@
 //   l = -inf where the row's mask has bit v clear
 //
 // Bound by memory: every logit is read and written once. A CTA takes a slice of one row's
-// vocabulary; it counts the row's history into a table of the slice in shared memory (integer
-// atomics: the result has no order) and streams the slice past it.
+// vocabulary, requests the whole slice (16 logits per thread) before anything else, and while
+// those loads are in flight counts the row's history into a table of the slice in shared memory
+// (integer atomics: the result has no order). A slice is as small as keeps the grid within one
+// round of CTAs, so that few rows still use many SMs; wide batches take the largest slice, where
+// the history is read least often.
 #include <algorithm>
 
 #include "orch_common.cuh"
@@ -19,9 +22,12 @@ namespace orch {
 
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpMaxSlice = 8192;
-constexpr uint32_t kLpSeen = 0x80000000u;  // top bit of a table word: seen; below it the count
+constexpr int kLpThreads = 512;
+constexpr int kLpEach = 16;  // logits per thread at most
+constexpr int kLpMaxSlice = kLpThreads * kLpEach;
+// A table word of the slice. Packed: count (15 bits), seen (bit 15), bias entry + 1 (16 bits).
+// Histories or bias lists too long for that take two words: seen and count, and the bias entry.
+constexpr int kLpPackedHist = 32767, kLpPackedBias = 65534;
 
 struct LpArgs {
   const void* in;
@@ -39,73 +45,144 @@ struct LpArgs {
   const uint32_t* masks;
   int mask_words, num_masks;
   const int* mask_rows;
-  int slice;
+  int slice, pieces;
   uint32_t* check;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads) logits_process_kernel(const LpArgs a) {
-  extern __shared__ uint32_t lp_tab[];  // [slice] seen and counts, then [slice] bias entries
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) LpVec {
+  T v[VEC];
+};
+
+// VEC: logits per load (16 bytes where rows are aligned for it, else one). WIDE: two-word table.
+template <typename T, int VEC, bool WIDE>
+__global__ void __launch_bounds__(kLpThreads, 3) logits_process_kernel(const LpArgs a) {
+  constexpr int P = kLpEach / VEC;
+  constexpr uint32_t kSeen = WIDE ? 0x80000000u : 0x8000u, kCount = kSeen - 1u;
+  extern __shared__ __align__(16) uint32_t lp_tab[];
   pdl_trigger();
   pdl_wait();
   const int m = blockIdx.y, i0 = blockIdx.x * a.slice, n = min(a.slice, a.V - i0), tid = threadIdx.x;
   const int hlen = a.hist ? a.hist_len[m] : 0, g0 = a.hist && a.gen_start ? a.gen_start[m] : 0;
   const int b0 = a.bias_ids ? a.bias_off[m] : 0, b1 = a.bias_ids ? a.bias_off[m + 1] : 0;
   const int mr = a.masks ? a.mask_rows[m] : -1;
+  const T* in = static_cast<const T*>(a.in) + (size_t)m * a.ld + i0;
+  LpVec<T, VEC> x[P];
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int i = (p * kLpThreads + tid) * VEC;
+    if (p < a.pieces) {
+      if (VEC == 1 || i + VEC <= n) {
+        if (i < n) x[p] = *reinterpret_cast<const LpVec<T, VEC>*>(in + i);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (i + e < n) x[p].v[e] = in[i + e];
+      }
+    }
+  }
   if (hlen < 0 || hlen > a.hist_ld || b0 < 0 || b1 < b0 || b1 > a.num_bias || mr >= a.num_masks) {
     if (tid == 0) atomicOr(a.check, 16u);
     return;
   }
   const bool pen = a.pen != nullptr && hlen > 0, bias = b1 > b0;
-  uint32_t* btab = lp_tab + a.slice;
+  uint32_t* btab = WIDE ? lp_tab + a.slice : lp_tab;
   if (pen || bias) {
-    for (int i = tid; i < n; i += kLpThreads) {
-      lp_tab[i] = 0u;
-      if (bias) btab[i] = 0u;
-    }
+    for (int i = tid * 4; i < a.slice * (WIDE ? 2 : 1); i += kLpThreads * 4)
+      *reinterpret_cast<uint4*>(lp_tab + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
-    const int lo = a.base + i0;
+    // ids as unsigned distances from the slice's first: one comparison, none below it passes
+    const uint32_t lo = (uint32_t)(a.base + i0), un = (uint32_t)n;
+    if (bias) {
+      for (int j = b0 + tid; j < b1; j += kLpThreads) {
+        const uint32_t v = (uint32_t)a.bias_ids[j] - lo;
+        if (v < un) atomicMax(&btab[v], (uint32_t)(j - b0 + 1) << (WIDE ? 0 : 16));
+      }
+      if (!WIDE) __syncthreads();  // the maximum is over words without counts
+    }
     if (pen) {
       const int* h = a.hist + (size_t)m * a.hist_ld;
-      for (int j = tid; j < hlen; j += kLpThreads) {
-        const int v = h[j];
-        if (v >= lo && v - lo < n) {
-          atomicOr(&lp_tab[v - lo], kLpSeen);
-          if (j >= g0) atomicAdd(&lp_tab[v - lo], 1u);
-        }
+      for (int j0 = tid; j0 < hlen; j0 += 4 * kLpThreads) {
+        uint32_t v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = j0 + u * kLpThreads < hlen ? (uint32_t)h[j0 + u * kLpThreads] - lo : un;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (v[u] < un) {
+            atomicOr(&lp_tab[v[u]], kSeen);
+            if (j0 + u * kLpThreads >= g0) atomicAdd(&lp_tab[v[u]], 1u);
+          }
       }
-    }
-    for (int j = b0 + tid; j < b1; j += kLpThreads) {
-      const int v = a.bias_ids[j];
-      if (v >= lo && v - lo < n) atomicMax(&btab[v - lo], (uint32_t)(j - b0 + 1));
     }
     __syncthreads();
   }
   const float rep = pen ? a.pen[3 * m] : 1.f, pres = pen ? a.pen[3 * m + 1] : 0.f, freq = pen ? a.pen[3 * m + 2] : 0.f;
   const uint32_t* mask = mr >= 0 ? a.masks + (size_t)mr * a.mask_words : nullptr;
-  const T* in = static_cast<const T*>(a.in) + (size_t)m * a.ld + i0;
   T* out = static_cast<T*>(a.out) + (size_t)m * a.ld + i0;
-  for (int i = tid; i < n; i += kLpThreads) {
-    float l = to_f32(in[i]);
-    if (pen) {
-      const uint32_t t = lp_tab[i];
-      if (t != 0u) {
-        l = l > 0.f ? l / rep : l * rep;
-        const uint32_t c = t & ~kLpSeen;
-        if (c != 0u) l -= fmaf(freq, (float)c, pres);
-      }
-    }
-    if (bias) {
-      const uint32_t t = btab[i];
-      if (t != 0u) l += a.bias_vals[b0 + t - 1];
-    }
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    const int i = (p * kLpThreads + tid) * VEC;
+    if (p >= a.pieces || i >= n) continue;
+    const uint32_t v0 = (uint32_t)(a.base + i0 + i);
+    // the mask bits of VEC ids from v0 on: a word, and the next one where they straddle
+    uint32_t ok = 0xffffffffu;
     if (mask != nullptr) {
-      const uint32_t v = (uint32_t)(a.base + i0 + i);
-      const uint32_t w = v >> 5;
-      if (!((w < (uint32_t)a.mask_words ? mask[w] : 0u) >> (v & 31u) & 1u)) l = -INFINITY;
+      const uint32_t w = v0 >> 5, s = v0 & 31u, nw = (uint32_t)a.mask_words;
+      const uint32_t lo_w = w < nw ? mask[w] : 0u, hi_w = s + VEC > 32 && w + 1 < nw ? mask[w + 1] : 0u;
+      ok = __funnelshift_r(lo_w, hi_w, s);
     }
-    out[i] = from_f32<T>(l);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float l = to_f32(x[p].v[e]);
+      if (pen || bias) {
+        const uint32_t t = i + e < n ? lp_tab[i + e] : 0u;
+        if (t & kSeen) {
+          l = l > 0.f ? l / rep : l * rep;
+          const uint32_t c = t & kCount;
+          if (c != 0u) l -= fmaf(freq, (float)c, pres);
+        }
+        const uint32_t b = WIDE ? (bias && i + e < n ? btab[i + e] : 0u) : t >> 16;
+        if (b != 0u) l += a.bias_vals[b0 + (int)b - 1];
+      }
+      if (!(ok >> e & 1u)) l = -INFINITY;
+      x[p].v[e] = from_f32<T>(l);
+    }
+    if (VEC == 1 || i + VEC <= n) {
+      *reinterpret_cast<LpVec<T, VEC>*>(out + i) = x[p];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e)
+        if (i + e < n) out[i + e] = x[p].v[e];
+    }
   }
+}
+
+template <typename T, int VEC, bool WIDE>
+int lp_launch(LpArgs a, cudaStream_t st) {
+  static bool attr_done[64] = {};
+  const int dev = device_index();
+  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    ORCH_CUDA(cudaFuncSetAttribute(logits_process_kernel<T, VEC, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   kLpMaxSlice * 4 * (WIDE ? 2 : 1)));
+    attr_done[dev] = true;
+  }
+  const uint64_t round = 3 * (uint64_t)num_sms(), unit = kLpThreads * VEC;
+  a.pieces = 1;
+  while (a.pieces < kLpEach / VEC && (a.V + unit * a.pieces - 1) / (unit * a.pieces) * a.M > round) ++a.pieces;
+  a.slice = (int)unit * a.pieces;
+  const dim3 grid((a.V + a.slice - 1) / a.slice, a.M), none(0, 0, 0);
+  const size_t smem = a.hist || a.bias_ids ? (size_t)a.slice * 4 * (WIDE ? 2 : 1) : 0;
+  ORCH_CUDA(launch_k(logits_process_kernel<T, VEC, WIDE>, grid, dim3(kLpThreads), smem, st, none, a));
+  return check_launch("logits_process");
+}
+
+template <typename T>
+int lp_dispatch(const LpArgs& a, cudaStream_t st) {
+  constexpr int V16 = 16 / sizeof(T);
+  const bool wide = a.hist_ld > kLpPackedHist || a.num_bias > kLpPackedBias;
+  const bool vec = a.ld % V16 == 0 && (((uintptr_t)a.in | (uintptr_t)a.out) & 15) == 0;
+  if (vec) return wide ? lp_launch<T, V16, true>(a, st) : lp_launch<T, V16, false>(a, st);
+  return wide ? lp_launch<T, 1, true>(a, st) : lp_launch<T, 1, false>(a, st);
 }
 
 }  // namespace
@@ -124,7 +201,7 @@ extern "C" int orch_logits_process(const void* logits, void* out, int dt, uint32
   if (M == 0) return ORCH_OK;
   ORCH_REQUIRE(logits && out && V > 0, "logits_process: null pointer or empty vocabulary");
   ORCH_REQUIRE(dt == ORCH_F32 || dt == ORCH_F16, "logits_process: bad dtype");
-  ORCH_REQUIRE(ld >= V && (uint64_t)base + V <= 0x7fffffffu, "logits_process: row stride below V, or ids out of range");
+  ORCH_REQUIRE(ld >= V && (uint64_t)base + V <= 0x7fff0000u, "logits_process: row stride below V, or ids out of range");
   ORCH_REQUIRE((history == nullptr) == (penalties == nullptr) && (!history || (hist_len && history_ld <= 0x7fffffffu)),
                "logits_process: penalties need history and hist_len (and history penalties)");
   ORCH_REQUIRE(!bias_ids || (bias_vals && bias_off && num_bias <= 0x7fffffffu),
@@ -140,7 +217,7 @@ extern "C" int orch_logits_process(const void* logits, void* out, int dt, uint32
   a.ld = (int)ld;
   a.base = (int)base;
   a.hist = history;
-  a.hist_ld = (int)history_ld;
+  a.hist_ld = history ? (int)history_ld : 0;
   a.hist_len = hist_len;
   a.gen_start = gen_start;
   a.pen = penalties;
@@ -152,22 +229,6 @@ extern "C" int orch_logits_process(const void* logits, void* out, int dt, uint32
   a.mask_words = (int)mask_words;
   a.num_masks = (int)num_masks;
   a.mask_rows = mask_rows;
-  // slices of whole mask words, enough of them for two CTAs per SM
-  const uint64_t per = ((uint64_t)M * V + 2 * num_sms() - 1) / (2 * num_sms());
-  a.slice = (int)(std::min<uint64_t>(std::max<uint64_t>(per, 512), kLpMaxSlice) + 31) / 32 * 32;
   ORCH_CHECK_WORD(a.check);
-  const dim3 grid((V + a.slice - 1) / a.slice, M), none(0, 0, 0);
-  const size_t smem = (size_t)a.slice * 4 * (bias_ids ? 2 : history ? 1 : 0);
-  static bool attr_done[64] = {};
-  const int dev = device_index();
-  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    ORCH_CUDA(cudaFuncSetAttribute(logits_process_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kLpMaxSlice * 4));
-    ORCH_CUDA(cudaFuncSetAttribute(logits_process_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kLpMaxSlice * 4));
-    attr_done[dev] = true;
-  }
-  if (dt == ORCH_F32)
-    ORCH_CUDA(launch_k(logits_process_kernel<float>, grid, dim3(kLpThreads), smem, as_stream(stream), none, a));
-  else
-    ORCH_CUDA(launch_k(logits_process_kernel<__half>, grid, dim3(kLpThreads), smem, as_stream(stream), none, a));
-  return check_launch("logits_process");
+  return dt == ORCH_F32 ? lp_dispatch<float>(a, as_stream(stream)) : lp_dispatch<__half>(a, as_stream(stream));
 }

@@ -509,3 +509,28 @@ def test_logits_skips_bad_rows():
         call("orch_logits_process", D(x), dout, F32, 3, 100, 100, 0, None, 0, None, None, None, D(np.zeros(3, np.int32)),
              D(np.zeros(3, np.float32)), D(np.array(off, np.int32)), 3, None, 0, 0, None, S())
         assert (dout[1] == 9).all() and flags() == 16
+
+
+@pytest.mark.parametrize("H,nb", [(40001, 3), (9, 70000)])
+def test_logits_long_lists(H, nb):
+    """Histories past 32,767 ids and bias lists past 65,534 entries: counts and list positions
+    that no longer fit half a table word."""
+    V = 70
+    g = rng(11, H)
+    x = g.standard_normal((2, V), dtype=np.float32)
+    hist = g.integers(0, V, (2, H)).astype(np.int32)
+    hist[0, 5:] = 7
+    n, gen = np.array([H, H - 2], np.int32), np.array([0, 3], np.int32)
+    pen = np.array([[1.25, 0.5, 2.0 ** -10]] * 2, np.float32)
+    bias = [[(int(v), float(np.float32(w))) for v, w in zip(g.integers(0, V, nb), g.standard_normal(nb))], [(3, 1.0)]]
+    got = run_logits(x, hist=hist, hist_len=n, gen=gen, pen=pen, bias=bias)
+    for m in range(2):
+        want = x[m].astype(np.float64)
+        ids, c = np.unique(hist[m, gen[m]:n[m]], return_counts=True)
+        seen = np.unique(hist[m, :n[m]])
+        want[seen] = np.where(want[seen] > 0, want[seen] / 1.25, want[seen] * 1.25)
+        want[ids] -= c * 2.0 ** -10 + 0.5
+        for v, b in dict(bias[m]).items():
+            want[v] += b
+        assert np.all(np.abs(got[m] - want) <= 2.0 ** -22 * (np.abs(want) + np.abs(x[m]) + 100))
+    assert flags() == 0
