@@ -22,43 +22,13 @@
 // (max, sum, O) meet in shared memory at the end, so few rows still keep every warp at work.
 // K and V blocks of 64 keys are copied by cp.async into a double buffer.
 #include <algorithm>
+#include <cstdlib>
 
-#include "orch_common.cuh"
+#include "attention_prefix.cuh"
 
 namespace orch {
 
 namespace {
-
-constexpr int kApKeys = 64;         // keys per block
-constexpr int kApMaxUnitRows = 128;  // rows of a unit
-constexpr uint32_t kApMaxLen = 1u << 29;  // entries of a slot: twice that stays an int
-constexpr float kApShift = 10.f;    // P is held as 2^10 e^(s - max)
-
-struct ApArgs {
-  const __half* q;
-  const __half* kp;
-  const __half* vp;
-  const int4* units;  // (row0, rows, prefix slot, prefix length)
-  int num_units, max_prefix, prefix_cap, num_prefix;
-  const __half* kc;
-  const __half* vc;
-  const int* lens;
-  const int* slots;
-  int max_own, max_seq, num_slots;
-  float* mass;
-  __half* out;
-  int M, nh, nkv, G;
-  int wr_p, wr_o;        // warps along the rows of a prefix tile / an own tile
-  int tiles_p, tiles_o;  // row tiles per unit / per row
-  int S_p, S_o;          // key ranges of a prefix / of a row's own entries
-  int blocks_p;          // CTAs of the prefix part (the first ones of the grid)
-  int direct;            // one range in all: the output is written by the attention kernel
-  float* acc;            // [M * nh][S][HD]
-  float2* stat;          // [M * nh][S]: (max, sum), in powers of two
-  float* scores;         // [M * nh][lds], with mass only
-  int lds;
-  uint32_t* check;
-};
 
 __device__ __forceinline__ void ap_cp16(void* dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
@@ -75,28 +45,11 @@ __device__ __forceinline__ void ap_ldsm4_t(const __half* p, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
 }
-__device__ __forceinline__ float ap_exp2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// Keys of range s of n keys cut into at most S ranges of whole blocks.
-__host__ __device__ __forceinline__ int ap_range(int n, int S) {
-  const int per = (n + S - 1) / S;
-  return (per + kApKeys - 1) / kApKeys * kApKeys;
-}
-
-// A unit that names rows, a prefix slot and a length inside what the call was given.
-__device__ __forceinline__ bool ap_unit_ok(const ApArgs& a, const int4& u) {
-  return u.y >= 1 && u.y <= kApMaxUnitRows && u.x >= 0 && u.x < a.M && u.y <= a.M - u.x && u.w >= 0 &&
-         u.w <= a.max_prefix && u.z >= 0 && u.z < a.num_prefix;
-}
-// The row's cache slot and own length, or false when either lies outside the cache.
-__device__ __forceinline__ bool ap_row(const ApArgs& a, int m, int& slot, int& len) {
-  slot = a.slots ? a.slots[m] : m;
-  len = a.lens[m];
-  return slot >= 0 && slot < a.num_slots && len >= 0 && len <= a.max_own;
+// Half-element offset of 16-byte piece c of row r in a tile of HD-wide rows: pieces are permuted
+// within 128 bytes so that the eight rows of an ldmatrix fall in distinct banks.
+template <int HD>
+__device__ __forceinline__ int ap_at(int r, int c) {
+  return r * HD + ((HD == 32 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 3);
 }
 
 // One tile: query rows i0 .. i0 + n - 1 of the (row, head of kv) pairs starting at row m0,
@@ -104,7 +57,7 @@ __device__ __forceinline__ bool ap_row(const ApArgs& a, int m, int& slot, int& l
 template <int HD, int WR>
 __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, int kv, const __half* kb,
                                         const __half* vb, int j0, int j1, int split, float* srow) {
-  constexpr int WK = 4 / WR, TR = 16 * WR, P = HD + 8, TILE = kApKeys * P, KT = kApKeys / 8 / WK;
+  constexpr int WK = 4 / WR, TR = 16 * WR, TILE = kApKeys * HD, KT = kApKeys / 8 / WK;
   extern __shared__ __align__(16) uint8_t ap_smem[];
   __half* buf = reinterpret_cast<__half*>(ap_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
@@ -117,11 +70,11 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
     constexpr int CPR = HD / 8;  // 16-byte pieces per row
 #pragma unroll
     for (int j = 0; j < kApKeys * CPR / 128; ++j) {
-      const int i = tid + 128 * j, r = i / CPR, d8 = (i % CPR) * 8, key = j0 + b * kApKeys + r;
+      const int i = tid + 128 * j, r = i / CPR, c8 = i % CPR, key = j0 + b * kApKeys + r;
       const bool ok = key < j1;
-      const size_t off = ok ? (size_t)key * HD + d8 : 0;
-      ap_cp16(kd + r * P + d8, kb + off, ok);
-      ap_cp16(vd + r * P + d8, vb + off, ok);
+      const size_t off = ok ? (size_t)key * HD + c8 * 8 : 0;
+      ap_cp16(kd + ap_at<HD>(r, c8), kb + off, ok);
+      ap_cp16(vd + ap_at<HD>(r, c8), vb + off, ok);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -130,23 +83,23 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
   // Q rows through buffer 1, then into registers as A fragments
   __half* qs = buf + 2 * TILE;
   for (int i = tid; i < TR * (HD / 8); i += 128) {
-    const int r = i / (HD / 8), d8 = (i % (HD / 8)) * 8;
+    const int r = i / (HD / 8), c8 = i % (HD / 8);
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (r < n) {
       const int m = m0 + (i0 + r) / a.G, h = kv * a.G + (i0 + r) % a.G;
-      v = *reinterpret_cast<const uint4*>(a.q + ((size_t)m * a.nh + h) * HD + d8);
+      v = *reinterpret_cast<const uint4*>(a.q + ((size_t)m * a.nh + h) * HD + c8 * 8);
     }
-    *reinterpret_cast<uint4*>(qs + r * P + d8) = v;
+    *reinterpret_cast<uint4*>(qs + ap_at<HD>(r, c8)) = v;
   }
   __syncthreads();
   const int qr = wrow * 16 + g;  // this thread's rows: qr and qr + 8
   uint32_t qa[HD / 16][4];
 #pragma unroll
   for (int kk = 0; kk < HD / 16; ++kk) {
-    qa[kk][0] = *reinterpret_cast<const uint32_t*>(qs + qr * P + 16 * kk + 2 * c);
-    qa[kk][1] = *reinterpret_cast<const uint32_t*>(qs + (qr + 8) * P + 16 * kk + 2 * c);
-    qa[kk][2] = *reinterpret_cast<const uint32_t*>(qs + qr * P + 16 * kk + 8 + 2 * c);
-    qa[kk][3] = *reinterpret_cast<const uint32_t*>(qs + (qr + 8) * P + 16 * kk + 8 + 2 * c);
+    qa[kk][0] = *reinterpret_cast<const uint32_t*>(qs + ap_at<HD>(qr, 2 * kk) + 2 * c);
+    qa[kk][1] = *reinterpret_cast<const uint32_t*>(qs + ap_at<HD>(qr + 8, 2 * kk) + 2 * c);
+    qa[kk][2] = *reinterpret_cast<const uint32_t*>(qs + ap_at<HD>(qr, 2 * kk + 1) + 2 * c);
+    qa[kk][3] = *reinterpret_cast<const uint32_t*>(qs + ap_at<HD>(qr + 8, 2 * kk + 1) + 2 * c);
   }
   __syncthreads();  // buffer 1 is free for block 1
 
@@ -176,7 +129,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 #pragma unroll
       for (int kk = 0; kk < HD / 16; kk += 2) {
         uint32_t bb[4];
-        ap_ldsm4(ks + (8 * (kt0 + t) + lr) * P + 16 * kk + 8 * lm, bb);
+        ap_ldsm4(ks + ap_at<HD>(8 * (kt0 + t) + lr, 2 * kk + lm), bb);
         mma_16816(sc[t], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bb[0], bb[1]);
         mma_16816(sc[t], qa[kk + 1][0], qa[kk + 1][1], qa[kk + 1][2], qa[kk + 1][3], bb[2], bb[3]);
       }
@@ -244,7 +197,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 #pragma unroll
       for (int d = 0; d < HD / 8; d += 2) {
         uint32_t bb[4];
-        ap_ldsm4_t(vs + (8 * kt0 + 16 * j + 8 * (lm & 1) + lr) * P + 8 * d + 8 * (lm >> 1), bb);
+        ap_ldsm4_t(vs + ap_at<HD>(8 * kt0 + 16 * j + 8 * (lm & 1) + lr, d + (lm >> 1)), bb);
         mma_16816(o[d], pa[0], pa[1], pa[2], pa[3], bb[0], bb[1]);
         mma_16816(o[d + 1], pa[0], pa[1], pa[2], pa[3], bb[2], bb[3]);
       }
@@ -319,25 +272,23 @@ __device__ __forceinline__ void ap_tile_wr(int wr, const ApArgs& a, int m0, int 
 }
 
 template <int HD>
-__global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
-  pdl_trigger();
-  pdl_wait();
+__device__ __forceinline__ void ap_work(const ApArgs& a) {
   int b = blockIdx.x;
   if (b < a.blocks_p) {  // a range of a prefix for a tile of the unit's query rows
     // row tiles fastest: the tiles that read the same keys run together
     const int tile = b % a.tiles_p;
     b /= a.tiles_p;
-    const int split = b % a.S_p;
-    b /= a.S_p;
-    const int kv = b % a.nkv;
-    const int4 u = a.units[b / a.nkv];
+    const int kv = b % a.nkv, split = b / a.nkv;
+    int4 u;
+    const int i0 = ap_find_tile(a, tile, u);
+    if (i0 < 0) return;
     if (!ap_unit_ok(a, u)) {
       if (threadIdx.x == 0) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
       return;
     }
-    const int tr = 16 * a.wr_p, i0 = tile * tr, n = min(tr, u.y * a.G - i0);
-    const int per = ap_range(u.w, a.S_p), j0 = split * per, j1 = min(u.w, j0 + per);
-    if (n <= 0 || j0 >= j1) return;
+    const int n = min(a.tr_p, u.y * a.G - i0);
+    const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
+    if (j0 >= j1) return;
     const size_t base = ((size_t)u.z * a.nkv + kv) * a.prefix_cap * HD;
     ap_tile_wr<HD>(a.wr_p, a, u.x, i0, n, kv, a.kp + base, a.vp + base, j0, j1, split, nullptr);
     return;
@@ -367,27 +318,42 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
   ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, a.kc + base, a.vc + base, j0, j1, a.S_p + split, srow);
 }
 
+template <int HD>
+__global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
+  pdl_trigger();
+  // Beside the prefix's own kernel, launched just before: that kernel waited for everything
+  // earlier before it let this one start, and the two share no output, so they run together.
+  // One CTA stays until it has ended, so that whoever waits for this grid waits for both.
+  if (!a.tc) pdl_wait();
+  ap_work<HD>(a);
+  if (a.tc && blockIdx.x == 0) pdl_wait();
+}
+
 // Ranges of row m that hold keys: prefix ranges 0 .. np - 1, own ranges S_p .. S_p + no - 1.
 // False when the row or its unit was rejected. (Called by whole warps.)
 __device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int& len, int& np, int& no) {
   const int lane = threadIdx.x & 31;
-  int plen = 0, bad = 0;
+  int plen = 0, bad = 0, in = 0;
   for (int u0 = 0; u0 < a.num_units; u0 += 32) {
     const int i = u0 + lane;
     if (i < a.num_units) {
       const int4 u = a.units[i];
       if (m >= u.x && (long long)m < (long long)u.x + u.y) {
-        if (ap_unit_ok(a, u))
+        if (ap_unit_ok(a, u)) {
           plen = max(plen, u.w);
-        else
+          ++in;
+        } else {
           bad = 1;
+        }
       }
     }
   }
   const bool ok = ap_row(a, m, slot, len);
   plen = __reduce_max_sync(0xffffffffu, plen);
-  if (__any_sync(0xffffffffu, bad) || !ok) return false;
-  np = plen > 0 ? (plen + ap_range(plen, a.S_p) - 1) / ap_range(plen, a.S_p) : 0;
+  in = (int)__reduce_add_sync(0xffffffffu, (unsigned)in);
+  if (in > 1 && lane == 0) atomicOr(a.check, 2u);  // in two units
+  if (__any_sync(0xffffffffu, bad) || !ok || in > 1) return false;
+  np = plen > 0 ? (plen + ap_range(plen, a.S_p, a.blk_p) - 1) / ap_range(plen, a.S_p, a.blk_p) : 0;
   no = len > 0 ? (len + ap_range(len, a.S_o) - 1) / ap_range(len, a.S_o) : 0;
   return true;
 }
@@ -539,10 +505,12 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
 
 // How a call is cut: rows per tile, key ranges, workspace. The same for the size query.
 struct ApPlan {
-  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, direct, lds;
+  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, blk_p, tr_p, tc, direct, lds;
   size_t acc_floats, stat_floats, score_floats;
   size_t bytes() const { return (acc_floats + stat_floats + score_floats) * sizeof(float); }
 };
+
+constexpr int kApTcFrom = 32;  // query rows of a unit above which its prefix takes the tcgen05 tiles
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
@@ -551,16 +519,36 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   ApPlan p;
   p.G = (int)(nh / nkv);
   const int rows_p = (int)std::min<uint32_t>(M, kApMaxUnitRows) * p.G;
+  const bool some = num_units > 0 && max_prefix > 0;
+  p.tc = some && hd != 32 && rows_p > kApTcFrom;
+  if (getenv("AP_TC")) p.tc = some && hd != 32 && rows_p > atoi(getenv("AP_TC"));
+  p.blk_p = p.tc ? kApTcKeys : kApKeys;
   p.wr_p = ap_wr(rows_p);
   p.wr_o = ap_wr(p.G);
-  p.tiles_p = (rows_p + 16 * p.wr_p - 1) / (16 * p.wr_p);
+  p.tr_p = p.tc ? kApTcRows : 16 * p.wr_p;
+  // the units share out at most M rows: their tiles are at most this many, and about `likely`
+  const size_t q_rows = (size_t)M * p.G;
+  p.tiles_p = some ? (int)((q_rows + (size_t)num_units * (p.tr_p - 1)) / p.tr_p) : 0;
+  const size_t likely = std::max<size_t>((q_rows + p.tr_p - 1) / p.tr_p, num_units);
   p.tiles_o = (p.G + 16 * p.wr_o - 1) / (16 * p.wr_o);
   const int want = 6 * num_sms();  // two rounds of three CTAs per SM
   const auto ranges = [&](size_t ctas, uint32_t keys, int least) {
     const size_t s = (want + ctas - 1) / std::max<size_t>(ctas, 1);
     return (int)std::max<size_t>(1, std::min<size_t>(s, (keys + least - 1) / least));
   };
-  p.S_p = num_units && max_prefix ? ranges((size_t)num_units * nkv * p.tiles_p, max_prefix, 64 * p.wr_p + 64) : 0;
+  const size_t items = nkv * likely;
+  p.S_p = 0;
+  if (p.tc) {
+    // one CTA per SM: the cut whose rounds cost least, a range's start and end counted as two blocks
+    const size_t blocks = (max_prefix + kApTcKeys - 1) / kApTcKeys, sms = num_sms();
+    size_t best = 0;
+    for (size_t s = 1; s <= std::min<size_t>(blocks, sms); ++s) {
+      const size_t cost = (items * s + sms - 1) / sms * ((blocks + s - 1) / s + 2);
+      if (p.S_p == 0 || cost < best) p.S_p = (int)s, best = cost;
+    }
+  } else if (some) {
+    p.S_p = ranges(items, max_prefix, 64 * p.wr_p + 64);
+  }
   p.S_o = ranges((size_t)M * nkv * p.tiles_o, max_own, 64);  // at least one: rows are checked there
   p.direct = p.S_p == 0 && p.S_o == 1 && !track;
   const size_t mh = (size_t)M * nh, S = p.S_p + p.S_o;
@@ -572,8 +560,8 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
 }
 
 template <int HD>
-int ap_launch(const ApArgs& a, cudaStream_t st) {
-  constexpr int kSmem = 4 * kApKeys * (HD + 8) * 2;
+int ap_launch(ApArgs a, cudaStream_t st) {
+  constexpr int kSmem = 4 * kApKeys * HD * 2;
   constexpr int kJoin = 64 * (HD + 4) * 4 + 64 * 8;  // WK x TR = 64 rows of O and their statistics
   constexpr int smem = kSmem > kJoin ? kSmem : kJoin;
   static bool attr_done[64] = {};
@@ -583,10 +571,14 @@ int ap_launch(const ApArgs& a, cudaStream_t st) {
     attr_done[dev] = true;
   }
   const dim3 none(0, 0, 0);
+  if (a.tc) {
+    const int rc = ap_tc_launch(a, HD, st);
+    if (rc != ORCH_OK) return rc;
+    a.blocks_p = 0;
+  }
   const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
-  if (blocks > 0)
-    ORCH_CUDA(launch_k_serial(attn_prefix_kernel<HD>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
+  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
   if (!a.direct) {
     const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
     const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
@@ -671,8 +663,13 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.tiles_p = p.tiles_p;
   a.tiles_o = p.tiles_o;
   a.S_p = p.S_p;
+  a.blk_p = p.blk_p;
+  a.tr_p = p.tr_p;
+  a.tc = p.tc;
   a.S_o = p.S_o;
-  const uint64_t blocks_p = (uint64_t)a.num_units * num_kv_heads * p.tiles_p * p.S_p;
+  const uint64_t blocks_p = (uint64_t)num_kv_heads * p.tiles_p * p.S_p;
+  if (p.tc && (uint64_t)num_prefix * num_kv_heads * prefix_cap > 0x7fffff00u)
+    return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: more than 2^31 prefix entries over all heads");
   if (blocks_p > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many units for one launch");
   a.blocks_p = (int)blocks_p;
   a.direct = p.direct;
