@@ -525,7 +525,7 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.blk_p = p.tc ? kApTcKeys : kApKeys;
   p.wr_p = ap_wr(rows_p);
   p.wr_o = ap_wr(p.G);
-  p.tr_p = p.tc ? kApTcRows : 16 * p.wr_p;
+  p.tr_p = !p.tc ? 16 * p.wr_p : rows_p > kApTcRows ? 2 * kApTcRows : kApTcRows;
   // the units share out at most M rows: their tiles are at most this many, and about `likely`
   const size_t q_rows = (size_t)M * p.G;
   p.tiles_p = some ? (int)((q_rows + (size_t)num_units * (p.tr_p - 1)) / p.tr_p) : 0;

@@ -93,7 +93,7 @@ __device__ __forceinline__ bool ap_row(const ApArgs& a, int m, int& slot, int& l
   return slot >= 0 && slot < a.num_slots && len >= 0 && len <= a.max_own;
 }
 
-// The prefix part on tcgen05 tiles of kApTcRows query rows (head_dim 64 or 128).
+// The prefix part on tcgen05 tiles of kApTcRows query rows, or twice as many (head_dim 64 or 128).
 constexpr int kApTcRows = 128, kApTcKeys = 128;
 int ap_tc_launch(const ApArgs& a, int hd, cudaStream_t st);
 

@@ -119,6 +119,29 @@ def test_prefix_rows_per_unit(rows, nh, nkv):
     check_attention(case(rows, 128, nh, nkv, [(0, rows, 0, 333)], lens, 40, pcap=340))
 
 
+@pytest.mark.parametrize("rows,nh,nkv,hd,plen", [(128, 32, 32, 128, 1777), (96, 32, 8, 64, 2500), (40, 160, 160, 64, 1300)])
+def test_prefix_of_many_blocks_per_range(rows, nh, nkv, hd, plen):
+    """Enough row tiles that one CTA goes through a long range; scores that grow along the keys,
+    so that the running scale has to move again and again."""
+    q, kp, vp, units, kc, vc, lens, slots = case(rows, hd, nh, nkv, [(0, rows, 0, plen)], [(3 * i) % 7 for i in range(rows)], 8, pcap=plen)
+    for k in (kp, kc):
+        k[...] = 0.25 * k + np.float16(0.5) * np.sign(q[0, 0, :]) * (np.arange(k.shape[2]) % 640 / 64)[:, None].astype(np.float16)
+    t = [D(x) for x in (q, kp, vp, units, kc, vc, lens, slots)]
+    out = attention(*t).double()
+    M, G = rows, nh // nkv
+    k, v = t[1][0, :, :plen].double(), t[2][0, :, :plen].double()
+    for m in range(0, M, 13):
+        n, s = int(lens[m]), int(slots[m])
+        kk, vv = torch.cat([k, t[4][s, :, :n].double()], 1), torch.cat([v, t[5][s, :, :n].double()], 1)
+        qq = t[0][m].double().view(nkv, G, hd)
+        p = torch.softmax(torch.einsum("kgd,kjd->kgj", qq, kk) / hd ** 0.5, -1)
+        want, absv = torch.einsum("kgj,kjd->kgd", p, vv), torch.einsum("kgj,kjd->kgd", p, vv.abs())
+        big = float(torch.einsum("kgd,kjd->kgj", qq.abs(), kk.abs()).max() / hd ** 0.5)
+        err = (out[m].view(nkv, G, hd) - want).abs()
+        assert (err <= 2.0 ** -11 * (want.abs() + absv) + 2.0 ** -19 * big * absv + 2.0 ** -24).all()
+    assert flags() == 0
+
+
 def test_several_units_and_rows_in_none():
     """Three units of different sizes and lengths (one of length 0, two with one prefix), rows
     before, between and after them without any, rows with nothing at all."""
