@@ -68,8 +68,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* vfull = kfull + 2;
   uint64_t* sready = vfull + 2;  // scores written: also, the K slot is free
   uint64_t* sread = sready + 2;  // scores read
-  uint64_t* pready = sread + 2;
-  uint64_t* pvdone = pready + 2;  // four, block i's at i & 3: weights used, the V slot is free
+  uint64_t* pready = sread + 2;   // [group][half]: weights of the block's first and last 64 keys
+  uint64_t* pvdone = pready + 4;  // four, block i's at i & 3: weights used, the V slot is free
   uint64_t* refset = pvdone + 4;  // [group][warp of the group]: the rows' ref after its block
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(refset + 8);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&vfull[i], 1);
       mbar_init(&sready[i], 1);
       mbar_init(&sread[i], 4);  // one lane per warp of the group
-      mbar_init(&pready[i], 4);
+      mbar_init(&pready[2 * i], 4);
+      mbar_init(&pready[2 * i + 1], 4);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&pvdone[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&refset[i], 1);
@@ -177,9 +178,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     auto wait = [&](uint64_t* bar, int phase) {
       return __all_sync(0xffffffffu, mbar_wait_f(bar, (uint32_t)phase & 1, failed)) != 0;
     };
+    // The waits for K and V (`arrived`) are placed where products are running, not before them.
+    auto arrived = [&](uint64_t* full, int i) { return i >= nb || wait(&full[i & 1], i >> 1); };
     // block i's scores into buffer g, from rows 128 g of the tile (PAIR) or all of them
     auto scores = [&](int g, int i) {
-      if (!wait(&kfull[i & 1], i >> 1)) return false;
       tc_fence_after();
       uint8_t* q = sm + (PAIR ? g * C::Tile : 0);
 #pragma unroll
@@ -188,38 +190,53 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                          sw128_desc(smem_u32(sK + (i & 1) * C::Tile + (kk >> 2) * C::Atom)) + 2 * (kk & 3), kIdescS, kk > 0);
       umma_commit_warp(&sready[g]);
       ++issued_s[g];
-      return true;
     };
-    auto weigh = [&](int g, int i, int done) {  // accumulator of g += weights of block i . V
-      // the last block's keys past the range: whole steps of 16 are left out
-      const int steps = min(kApTcKeys, (j1 - j0 - i * kApTcKeys + 15) / 16 * 16) / 16;
-      tc_fence_after();
+    // accumulator of g += weights of block i . V, as the two halves of the weights come
+    auto weigh = [&](int g, int i, int done) {
+      const uint32_t d = tmem + C::ColO + g * C::StepO, p = tmem + C::ColP + g * C::StepP;
+      const uint64_t v = sw128_desc_mn(smem_u32(sV + (i & 1) * C::Tile), C::Atom);  // 16 keys are 2,048 B
+      const int steps = (min(kApTcKeys, j1 - j0 - i * kApTcKeys) + 15) / 16, phase = PAIR ? i : i >> 1;
 #pragma unroll
-      for (int kk = 0; kk < kApTcKeys / 16; ++kk)
-        if (kk < steps)
-          umma_f16_ta_warp(tmem + C::ColO + g * C::StepO, tmem + C::ColP + g * C::StepP + kk * 8,
-                           sw128_desc_mn(smem_u32(sV + (i & 1) * C::Tile + kk * 2048), C::Atom), kIdescO, i > 0 || kk > 0);
+      for (int h = 0; h < 2; ++h) {
+        if (!wait(&pready[2 * g + h], phase)) return false;
+        tc_fence_after();
+        if (steps >= 4 * h + 4) {
+#pragma unroll
+          for (int kk = 4 * h; kk < 4 * h + 4; ++kk) umma_f16_ta_warp(d, p + kk * 8, v + kk * 128, kIdescO, i > 0 || kk > 0);
+        } else {  // the last block: steps of 16 keys past the range are left out
+          for (int kk = 4 * h; kk < steps; ++kk) umma_f16_ta_warp(d, p + kk * 8, v + kk * 128, kIdescO, i > 0 || kk > 0);
+        }
+      }
       umma_commit_warp(&pvdone[done]);
       ++issued_o[done];
+      return true;
     };
-    bool ok = scores(0, 0);
+    bool ok = arrived(kfull, 0);
+    if (ok) scores(0, 0);
     if (PAIR) {
-      ok = ok && (groups < 2 || scores(1, 0));
+      if (ok && groups > 1) scores(1, 0);
+      ok = ok && arrived(vfull, 0);
       for (int i = 0; ok && i < nb; ++i)
         for (int g = 0; ok && g < groups; ++g) {
-          ok = wait(&pready[g], i) && wait(&vfull[i & 1], i >> 1);
-          if (!ok) break;
-          weigh(g, i, g);
+          ok = weigh(g, i, g) && (g > 0 || arrived(kfull, i + 1));
+          if (!ok || i + 1 >= nb) continue;
           // the next scores overwrite the weights: wait until they have been used
-          if (i + 1 < nb) ok = wait(&pvdone[g], i) && scores(g, i + 1);
+          ok = wait(&pvdone[g], i);
+          if (!ok) break;
+          scores(g, i + 1);
+          if (g == groups - 1) ok = arrived(vfull, i + 1);
         }
     } else {
-      ok = ok && (nb < 2 || scores(1, 1));
+      ok = ok && arrived(kfull, 1);
+      if (ok && nb > 1) scores(1, 1);
+      ok = ok && arrived(vfull, 0);
       for (int i = 0; ok && i < nb; ++i) {
         const int w = i & 1;
-        if (i + 2 < nb) ok = wait(&sread[w], i >> 1) && scores(w, i + 2);
-        ok = ok && wait(&pready[w], i >> 1) && wait(&vfull[w], i >> 1);
-        if (ok) weigh(w, i, i & 3);
+        if (i + 2 < nb) {
+          ok = arrived(kfull, i + 2) && wait(&sread[w], i >> 1);
+          if (ok) scores(w, i + 2);
+        }
+        ok = ok && weigh(w, i, i & 3) && arrived(vfull, i + 1);
       }
     }
     if (!ok) {  // products still running
@@ -305,44 +322,38 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ref = now;
       const float off = now == -INFINITY ? 0.f : now - kPtShift;
       float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      bool good = true;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t p[8];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[32];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int x = 16 * c + 2 * e;
-          const float p0 = ap_exp2(fmaf(__uint_as_float(s[x >> 6][x & 63]), scale, -off));
-          const float p1 = ap_exp2(fmaf(__uint_as_float(s[x >> 6][(x & 63) + 1]), scale, -off));
+        for (int e = 0; e < 32; ++e) {
+          const float p0 = ap_exp2(fmaf(__uint_as_float(s[h][2 * e]), scale, -off));
+          const float p1 = ap_exp2(fmaf(__uint_as_float(s[h][2 * e + 1]), scale, -off));
           sum[(2 * e) & 3] += p0;
           sum[(2 * e + 1) & 3] += p1;
           p[e] = h2_bits(__floats2half2_rn(p0, p1));
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[c >> 2][(8 * c & 31) + e] = p[e];  // over scores already used
+        tmem_st32(tp + 32 * h, p);
+        if (h == 0 && keys < kApTcKeys) {  // the V rows of the last step that lie past the range
+          good = wait(&vfull[i & 1], i >> 1);
+          if (!good) break;
+          const int end = (keys + 15) / 16 * 16, pieces = (end - keys) * (HD / 8);
+          for (int x = row; x < pieces; x += 128) {
+            const int r = keys + x / (HD / 8), c = x % (HD / 8);
+            *reinterpret_cast<uint4*>(sV + (i & 1) * C::Tile + (c >> 3) * C::Atom + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pready[2 * grp + h]);
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) p[e] = s[c][e];
-        tmem_st32(tp + 32 * c, p);
+      if (!good) {
+        *failed = 1;
+        break;
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (keys < kApTcKeys) {  // the V rows of the last step that lie past the range
-        if (!wait(&vfull[i & 1], i >> 1)) {
-          *failed = 1;
-          break;
-        }
-        const int end = (keys + 15) / 16 * 16, pieces = (end - keys) * (HD / 8);
-        for (int x = row; x < pieces; x += 128) {
-          const int r = keys + x / (HD / 8), c = x % (HD / 8);
-          *reinterpret_cast<uint4*>(sV + (i & 1) * C::Tile + (c >> 3) * C::Atom + r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
-        fence_proxy_async();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&pready[grp]);
     }
     if (mine > 0 && !product(PAIR ? nb - 1 : 2 * mine - 2 + grp)) *failed = 1;
     tc_fence_before();
