@@ -380,7 +380,8 @@ __device__ __forceinline__ float2 ap_total(const ApArgs& a, size_t mh, int np, i
 
 // Joins the ranges: one warp per (row, head) for the output; with mass, further CTAs each
 // take kMassEntries entries of one (row, K/V head).
-constexpr int kMassEntries = 1024;
+constexpr int kMassEntries = 512;
+constexpr int kMassHeads = 32;  // heads whose totals are held at once
 
 template <int HD>
 __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, int blocks_out, int chunks) {
@@ -458,6 +459,7 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
   int slot, len, np, no;
   if (!ap_ranges(a, m, slot, len, np, no)) return;
   __shared__ int any;
+  __shared__ float2 tots[kMassHeads];
   if (threadIdx.x == 0) any = 0;
   __syncthreads();
   int mine = 0;  // whether another row of the call has this slot: 1 an earlier one, 2 a later one
@@ -484,15 +486,25 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
     float w[kMassEntries / 128];
 #pragma unroll
     for (int i = 0; i < kMassEntries / 128; ++i) w[i] = 0.f;
-    for (int h = kv * a.G; h < (kv + 1) * a.G; ++h) {
-      const size_t mh = (size_t)r * a.nh + h;
-      const float2 tot = ap_total(a, mh, np, no);
-      const float ref = tot.x == -INFINITY ? 0.f : tot.x - kApShift, inv = tot.y == 0.f ? 0.f : 1.0f / tot.y;
-      const float* sr = a.scores + mh * a.lds;
+    for (int h0 = 0; h0 < a.G; h0 += kMassHeads) {
+      const int hs = min(kMassHeads, a.G - h0);
+      __syncthreads();  // the totals of the heads before are done with
+      for (int j = warp; j < hs; j += 4) {  // the heads' totals, a warp each
+        const float2 tot = ap_total(a, (size_t)r * a.nh + kv * a.G + h0 + j, np, no);
+        if (lane == 0) tots[j] = make_float2(tot.x == -INFINITY ? 0.f : tot.x - kApShift, tot.y == 0.f ? 0.f : 1.0f / tot.y);
+      }
+      __syncthreads();
+      for (int j = 0; j < hs; ++j) {
+        const float2 tot = tots[j];
+        const float* sr = a.scores + ((size_t)r * a.nh + kv * a.G + h0 + j) * a.lds;
+        float sv[kMassEntries / 128];
 #pragma unroll
-      for (int i = 0; i < kMassEntries / 128; ++i) {
-        const int e = e0 + threadIdx.x + 128 * i;
-        if (e < len) w[i] = fmaf(ap_exp2(sr[e] - ref), inv, w[i]);
+        for (int i = 0; i < kMassEntries / 128; ++i) {
+          const int e = e0 + threadIdx.x + 128 * i;
+          sv[i] = e < len ? sr[e] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kMassEntries / 128; ++i) w[i] = fmaf(ap_exp2(sv[i] - tot.x), tot.y, w[i]);
       }
     }
 #pragma unroll

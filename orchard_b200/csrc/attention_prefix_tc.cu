@@ -71,7 +71,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* pready = sread + 2;   // [group][half]: weights of the block's first and last 64 keys
   uint64_t* pvdone = pready + 4;  // four, block i's at i & 3: weights used, the V slot is free
   uint64_t* refset = pvdone + 4;  // [group][warp of the group]: the rows' ref after its block
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(refset + 8);
+  uint64_t* qfull = refset + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   float* refs = reinterpret_cast<float*>(sm + C::OffRef);
@@ -109,20 +110,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     for (int i = 0; i < 4; ++i) mbar_init(&pvdone[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&refset[i], 1);
+    mbar_init(qfull, 8);  // one lane per warp of the groups
     *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // Q rows into their swizzled places: 16-byte piece c of a 128-byte row r at c ^ (r & 7)
-  for (int i = tid; i < C::Rows * (HD / 8); i += kPtThreads) {
-    const int r = i / (HD / 8), c = i % (HD / 8);
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (r < n) {
-      const int m = u.x + (i0 + r) / a.G, h = kv * a.G + (i0 + r) % a.G;
-      v = *reinterpret_cast<const uint4*>(a.q + ((size_t)m * a.nh + h) * HD + c * 8);
-    }
-    *reinterpret_cast<uint4*>(sm + (r >> 7) * C::Tile + (c >> 3) * C::Atom + (r & 127) * 128 + ((c & 7) ^ (r & 7)) * 16) = v;
-  }
-  fence_proxy_async();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -211,7 +202,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ++issued_o[done];
       return true;
     };
-    bool ok = arrived(kfull, 0);
+    bool ok = arrived(kfull, 0) && wait(qfull, 0);
     if (ok) scores(0, 0);
     if (PAIR) {
       if (ok && groups > 1) scores(1, 0);
@@ -248,6 +239,32 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     __syncwarp();
   } else {
+    // Q rows into their swizzled places: 16-byte piece c of a 128-byte row r at c ^ (r & 7).
+    // Up to eight pieces per thread are requested before the first is stored.
+    constexpr int Pieces = C::Rows * (HD / 8) / 256, Batch = Pieces < 8 ? Pieces : 8;
+    static_assert(C::Rows * (HD / 8) % (256 * Batch) == 0, "whole batches");
+#pragma unroll
+    for (int x0 = 0; x0 < Pieces; x0 += Batch) {
+      uint4 v[Batch];
+#pragma unroll
+      for (int x = 0; x < Batch; ++x) {
+        const int i = tid + (x0 + x) * 256, r = i / (HD / 8), c = i % (HD / 8);
+        v[x] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < n) {
+          const int m = u.x + (i0 + r) / a.G, h = kv * a.G + (i0 + r) % a.G;
+          v[x] = *reinterpret_cast<const uint4*>(a.q + ((size_t)m * a.nh + h) * HD + c * 8);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < Batch; ++x) {
+        const int i = tid + (x0 + x) * 256, r = i / (HD / 8), c = i % (HD / 8);
+        *reinterpret_cast<uint4*>(sm + (r >> 7) * C::Tile + (c >> 3) * C::Atom + (r & 127) * 128 + ((c & 7) ^ (r & 7)) * 16) = v[x];
+      }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(qfull);
+
     const float scale = rsqrtf((float)HD) * 1.4426950408889634f;  // scores in powers of two
     const uint32_t ts = tmem + lanes + grp * 128, tp = tmem + lanes + C::ColP + grp * C::StepP,
                    to = tmem + lanes + C::ColO + grp * C::StepO;
@@ -382,23 +399,25 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     pt_groups_sync();
     constexpr int LPR = HD / 4;  // threads per row, four values each
     const int S = a.S_p + a.S_o;
-    for (int i = tid; i < n * LPR && good; i += 256) {
+    // the other kernels' records hold weights as 2^kApShift e^(s - max): the same scale here
+    const float g = exp2f(kApShift - kPtShift);
+#pragma unroll 4
+    for (int i = tid; i < (good ? n * LPR : 0); i += 256) {
       const int r = i / LPR, d = (i % LPR) * 4;
-      // the other kernels' records hold weights as 2^kApShift e^(s - max): the same scale here
-      const float g = exp2f(kApShift - kPtShift);
-      const size_t mh = (size_t)(u.x + (i0 + r) / a.G) * a.nh + kv * a.G + (i0 + r) % a.G;
+      const size_t rec = ((size_t)(u.x + (i0 + r) / a.G) * a.nh + kv * a.G + (i0 + r) % a.G) * S + split;
       const float4 ov = *reinterpret_cast<const float4*>(os + r * C::OP + d);
-      *reinterpret_cast<float4*>(a.acc + (mh * S + split) * HD + d) = make_float4(ov.x * g, ov.y * g, ov.z * g, ov.w * g);
-      if (d == 0) {
-        float2 st = ss[r];
-        if (!PAIR) {  // the groups' sums, at the last block's ref
-          const float at = refs[r];
-          const float2 s1 = nb > 1 ? ss[kApTcRows + r] : make_float2(at, 0.f);
-          st.y = (st.x == at ? st.y : st.y * ap_exp2(st.x - at)) + (s1.x == at ? s1.y : s1.y * ap_exp2(s1.x - at));
-          st.x = at;
-        }
-        a.stat[mh * S + split] = make_float2(st.x, st.y * g);
+      *reinterpret_cast<float4*>(a.acc + rec * HD + d) = make_float4(ov.x * g, ov.y * g, ov.z * g, ov.w * g);
+    }
+    if (good && tid < n) {
+      const int r = tid;
+      float2 st = ss[r];
+      if (!PAIR) {  // the groups' sums, at the last block's ref
+        const float at = refs[r];
+        const float2 s1 = nb > 1 ? ss[kApTcRows + r] : make_float2(at, 0.f);
+        st.y = (st.x == at ? st.y : st.y * ap_exp2(st.x - at)) + (s1.x == at ? s1.y : s1.y * ap_exp2(s1.x - at));
+        st.x = at;
       }
+      a.stat[((size_t)(u.x + (i0 + r) / a.G) * a.nh + kv * a.G + (i0 + r) % a.G) * S + split] = make_float2(st.x, st.y * g);
     }
   }
   tc_fence_before();
