@@ -325,6 +325,20 @@ int orch_attention_prefix(const void* q, const void* prefix_k, const void* prefi
                           uint32_t max_own, uint32_t max_seq, uint32_t num_slots, float* mass, void* out, uint32_t M,
                           uint32_t num_heads, uint32_t num_kv_heads, uint32_t head_dim, void* workspace,
                           size_t workspace_bytes, void* stream);
+/* orch_q4t_qkv_rope and orch_q4t_rms_qkv_rope with the rotation and the place apart: row m's
+ * q and k are rotated for position pos[m] (< max_pos), k and v go to entry index[m] (< max_seq)
+ * of its slot. A cache that does not hold every position (entries evicted, a prefix held
+ * elsewhere) has its next free entry below the token's position. */
+int orch_q4t_qkv_rope_at(const void* tiled_qkv, const void* x, uint32_t M, uint32_t K, uint32_t H,
+                         uint32_t num_heads, const int32_t* pos, const int32_t* index, const int32_t* slots,
+                         const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
+                         void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots,
+                         const float* lora_t, const float* lora_b, uint32_t lora_r, void* stream);
+int orch_q4t_rms_qkv_rope_at(const void* tiled_qkv, const float* x, const float* norm_w, float eps,
+                             void* xn, uint32_t M, uint32_t K, uint32_t H, uint32_t num_heads,
+                             const int32_t* pos, const int32_t* index, const int32_t* slots,
+                             const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
+                             void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots, void* stream);
 /* Drops cache entries by accumulated weight. Each (row, K/V head) keeps n = min(lens[m], budget)
  * of its lens[m] entries: the protected ones first (positions[e] > the row and head's largest
  * position - recent), then by mass, equal masses by the lower index (a NaN is the smallest

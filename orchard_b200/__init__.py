@@ -1,6 +1,8 @@
 """orchard_b200: Orchard's quantised Llama-layer path on NVIDIA B200 (sm_100a).
 
 * ``orchard_b200.Llama`` -- ``orchard.Llama`` (orchard/model.py:197-381) on fused CUDA kernels.
+* ``orchard_b200.BatchServer`` -- batches with a shared prefix, a bounded cache and controlled
+  logits on the same engine.
 * ``orchard_b200.quantize_q4_0`` -- the reference packer (orchard/quantizer.py:3-78).
 * ``orchard_b200.orchard_core`` -- the reference's pybind11 operator surface
   (src/bindings.cpp) over the same kernels; ``install_as_orchard_core()`` registers it
@@ -23,6 +25,9 @@ def __getattr__(name):
     if name in ("Llama", "LlamaConfig", "DecodeEngine", "precompute_freqs_cis"):
         from . import model
         return getattr(model, name)
+    if name in ("BatchServer", "LogitsControls", "SharedPrefix"):
+        from . import serving
+        return getattr(serving, name)
     if name == "orchard_core":
         return importlib.import_module(".orchard_core", __name__)
     raise AttributeError(name)

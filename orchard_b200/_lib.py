@@ -102,6 +102,10 @@ _SIGS = {
     "orch_attention_prefix_workspace_bytes": (_sz, [_u32, _u32, _u32, _u32, _u32, _u32, _u32, _i32]),
     "orch_attention_prefix": (_i32, [_vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _u32, _u32, _u32,
                                      _vp, _vp, _u32, _u32, _u32, _u32, _vp, _sz, _vp]),
+    "orch_q4t_qkv_rope_at": (_i32, [_vp, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _u32,
+                                    _vp, _vp, _vp, _u32, _u32, _vp, _vp, _u32, _vp]),
+    "orch_q4t_rms_qkv_rope_at": (_i32, [_vp, _vp, _vp, _f32, _vp, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _vp, _u32,
+                                        _vp, _vp, _vp, _u32, _u32, _vp]),
     "orch_cache_evict": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
                                 _vp]),
     "orch_logits_process": (_i32, [_vp, _vp, _i32, _u32, _u32, _u32, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _u32,

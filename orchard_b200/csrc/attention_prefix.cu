@@ -22,7 +22,6 @@
 // (max, sum, O) meet in shared memory at the end, so few rows still keep every warp at work.
 // K and V blocks of 64 keys are copied by cp.async into a double buffer.
 #include <algorithm>
-#include <cstdlib>
 
 #include "attention_prefix.cuh"
 
@@ -533,7 +532,6 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   const int rows_p = (int)std::min<uint32_t>(M, kApMaxUnitRows) * p.G;
   const bool some = num_units > 0 && max_prefix > 0;
   p.tc = some && hd != 32 && rows_p > kApTcFrom;
-  if (getenv("AP_TC")) p.tc = some && hd != 32 && rows_p > atoi(getenv("AP_TC"));
   p.blk_p = p.tc ? kApTcKeys : kApKeys;
   p.wr_p = ap_wr(rows_p);
   p.wr_o = ap_wr(p.G);

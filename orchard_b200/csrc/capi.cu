@@ -320,10 +320,10 @@ static int linear_swiglu(const void* w13, const void* s13, bool tiled, const voi
 }
 
 static int qkv_rope(const void* wqkv, const void* sqkv, bool tiled, const void* x, uint32_t M, uint32_t K, uint32_t H,
-                    uint32_t num_heads, const int32_t* pos, const int32_t* slots, const float* cos_tab,
-                    const float* sin_tab, uint32_t max_pos, void* q_out, void* k_cache, void* v_cache,
-                    uint32_t max_seq, uint32_t num_slots, const float* lora_t, const float* lora_b, uint32_t lora_r,
-                    void* stream) {
+                    uint32_t num_heads, const int32_t* pos, const int32_t* index, const int32_t* slots,
+                    const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out, void* k_cache,
+                    void* v_cache, uint32_t max_seq, uint32_t num_slots, const float* lora_t, const float* lora_b,
+                    uint32_t lora_r, void* stream) {
   if (M == 0) return ORCH_OK;
   int rc = check_q4w(wqkv, sqkv, x, K, tiled);
   if (rc) return rc;
@@ -345,6 +345,7 @@ static int qkv_rope(const void* wqkv, const void* sqkv, bool tiled, const void* 
   a.num_slots = (int)num_slots;
   a.max_pos = (int)max_pos;
   a.pos = pos;
+  a.cidx = index;
   a.slots = slots;
   a.cos_tab = cos_tab;
   a.sin_tab = sin_tab;
@@ -371,8 +372,8 @@ extern "C" int orch_q4_qkv_rope(const void* wqkv, const void* sqkv, const void* 
                                 const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
                                 void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots,
                                 const float* lora_t, const float* lora_b, uint32_t lora_r, void* stream) {
-  return qkv_rope(wqkv, sqkv, false, x, M, K, H, num_heads, pos, slots, cos_tab, sin_tab, max_pos, q_out, k_cache,
-                  v_cache, max_seq, num_slots, lora_t, lora_b, lora_r, stream);
+  return qkv_rope(wqkv, sqkv, false, x, M, K, H, num_heads, pos, nullptr, slots, cos_tab, sin_tab, max_pos, q_out,
+                  k_cache, v_cache, max_seq, num_slots, lora_t, lora_b, lora_r, stream);
 }
 
 // ---- tiled-layout forms (weights re-laid by orch_q4t_pack) ----------------------------------
@@ -408,7 +409,17 @@ extern "C" int orch_q4t_qkv_rope(const void* tiled_qkv, const void* x, uint32_t 
                                  const float* sin_tab, uint32_t max_pos, void* q_out, void* k_cache, void* v_cache,
                                  uint32_t max_seq, uint32_t num_slots, const float* lora_t, const float* lora_b,
                                  uint32_t lora_r, void* stream) {
-  return qkv_rope(tiled_qkv, nullptr, true, x, M, K, H, num_heads, pos, slots, cos_tab, sin_tab, max_pos, q_out,
+  return qkv_rope(tiled_qkv, nullptr, true, x, M, K, H, num_heads, pos, nullptr, slots, cos_tab, sin_tab, max_pos,
+                  q_out, k_cache, v_cache, max_seq, num_slots, lora_t, lora_b, lora_r, stream);
+}
+
+extern "C" int orch_q4t_qkv_rope_at(const void* tiled_qkv, const void* x, uint32_t M, uint32_t K, uint32_t H,
+                                    uint32_t num_heads, const int32_t* pos, const int32_t* index, const int32_t* slots,
+                                    const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
+                                    void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots,
+                                    const float* lora_t, const float* lora_b, uint32_t lora_r, void* stream) {
+  ORCH_REQUIRE(M == 0 || index, "q4t_qkv_rope_at: null index");
+  return qkv_rope(tiled_qkv, nullptr, true, x, M, K, H, num_heads, pos, index, slots, cos_tab, sin_tab, max_pos, q_out,
                   k_cache, v_cache, max_seq, num_slots, lora_t, lora_b, lora_r, stream);
 }
 
@@ -426,11 +437,10 @@ static int rms_args(QArgs& a, const float* x, const float* norm_w, float eps) {
   return ORCH_OK;
 }
 
-extern "C" int orch_q4t_rms_qkv_rope(const void* tiled_qkv, const float* x, const float* norm_w, float eps, void* xn,
-                                     uint32_t M, uint32_t K, uint32_t H, uint32_t num_heads, const int32_t* pos,
-                                     const int32_t* slots, const float* cos_tab, const float* sin_tab,
-                                     uint32_t max_pos, void* q_out, void* k_cache, void* v_cache, uint32_t max_seq,
-                                     uint32_t num_slots, void* stream) {
+static int rms_qkv_rope(const void* tiled_qkv, const float* x, const float* norm_w, float eps, void* xn, uint32_t M,
+                        uint32_t K, uint32_t H, uint32_t num_heads, const int32_t* pos, const int32_t* index,
+                        const int32_t* slots, const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
+                        void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots, void* stream) {
   if (M == 0) return ORCH_OK;
   ORCH_REQUIRE(xn, "rms_qkv_rope: null xn");
   if (M <= gemv_tiled_limit()) {
@@ -454,6 +464,7 @@ extern "C" int orch_q4t_rms_qkv_rope(const void* tiled_qkv, const float* x, cons
     a.num_slots = (int)num_slots;
     a.max_pos = (int)max_pos;
     a.pos = pos;
+    a.cidx = index;
     a.slots = slots;
     a.cos_tab = cos_tab;
     a.sin_tab = sin_tab;
@@ -464,8 +475,28 @@ extern "C" int orch_q4t_rms_qkv_rope(const void* tiled_qkv, const float* x, cons
   }
   int rc = orch_rmsnorm_ex(x, ORCH_F32, norm_w, ORCH_F32, xn, ORCH_F16, eps, K, M, stream);
   if (rc) return rc;
-  return orch_q4t_qkv_rope(tiled_qkv, xn, M, K, H, num_heads, pos, slots, cos_tab, sin_tab, max_pos, q_out, k_cache,
-                           v_cache, max_seq, num_slots, nullptr, nullptr, 0, stream);
+  return qkv_rope(tiled_qkv, nullptr, true, xn, M, K, H, num_heads, pos, index, slots, cos_tab, sin_tab, max_pos, q_out,
+                  k_cache, v_cache, max_seq, num_slots, nullptr, nullptr, 0, stream);
+}
+
+extern "C" int orch_q4t_rms_qkv_rope(const void* tiled_qkv, const float* x, const float* norm_w, float eps, void* xn,
+                                     uint32_t M, uint32_t K, uint32_t H, uint32_t num_heads, const int32_t* pos,
+                                     const int32_t* slots, const float* cos_tab, const float* sin_tab,
+                                     uint32_t max_pos, void* q_out, void* k_cache, void* v_cache, uint32_t max_seq,
+                                     uint32_t num_slots, void* stream) {
+  return rms_qkv_rope(tiled_qkv, x, norm_w, eps, xn, M, K, H, num_heads, pos, nullptr, slots, cos_tab, sin_tab, max_pos,
+                      q_out, k_cache, v_cache, max_seq, num_slots, stream);
+}
+
+extern "C" int orch_q4t_rms_qkv_rope_at(const void* tiled_qkv, const float* x, const float* norm_w, float eps,
+                                        void* xn, uint32_t M, uint32_t K, uint32_t H, uint32_t num_heads,
+                                        const int32_t* pos, const int32_t* index, const int32_t* slots,
+                                        const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
+                                        void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots,
+                                        void* stream) {
+  ORCH_REQUIRE(M == 0 || index, "q4t_rms_qkv_rope_at: null index");
+  return rms_qkv_rope(tiled_qkv, x, norm_w, eps, xn, M, K, H, num_heads, pos, index, slots, cos_tab, sin_tab, max_pos,
+                      q_out, k_cache, v_cache, max_seq, num_slots, stream);
 }
 
 extern "C" int orch_q4t_rms_linear_swiglu(const void* tiled13, const float* x, const float* norm_w, float eps,

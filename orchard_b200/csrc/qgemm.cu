@@ -373,6 +373,7 @@ int qgemm_run(QArgs a, cudaStream_t st) {
     } else {
       b.out = static_cast<__half*>(a.out) + (size_t)m0 * a.H;
       b.pos = a.pos + m0;
+      if (a.cidx) b.cidx = a.cidx + m0;
       if (a.slots) b.slots = a.slots + m0;
       else b.slot0 = a.slot0 + m0;
     }

@@ -44,6 +44,7 @@ struct QArgs {
   int H, nh, hd, max_seq, max_pos;
   uint32_t hd_magic;  // ceil(2^32 / hd): rr / hd = umulhi(rr, hd_magic) for rr, hd < 2^16
   const int* pos;
+  const int* cidx;    // cache entry of each row; null: its position
   const int* slots;   // cache slot of each row; null: row index (slot0 + local row)
   int slot0;          // with null slots, the first row's index (row blocks advance it)
   int num_slots;      // slots in the caches: a row whose slot is outside [0, num_slots) is skipped
@@ -224,8 +225,8 @@ __device__ __forceinline__ void epi_apply(const QArgs& a, int n, int idx, float 
       v0 += d0;
       v1 += d1;
     }
-    const int p = a.pos[n];
-    if (p < 0 || p >= a.max_seq || p >= a.max_pos) {
+    const int p = a.pos[n], entry = a.cidx != nullptr ? a.cidx[n] : p;
+    if (p < 0 || p >= a.max_pos || entry < 0 || entry >= a.max_seq) {
       atomicOr(a.check, 1u);
       return;
     }
@@ -247,7 +248,7 @@ __device__ __forceinline__ void epi_apply(const QArgs& a, int n, int idx, float 
         return;
       }
       __half* cache = region == 1 ? a.kc : a.vc;
-      const size_t off = (((size_t)slot * a.nh + head) * a.max_seq + p) * a.hd + d;
+      const size_t off = (((size_t)slot * a.nh + head) * a.max_seq + entry) * a.hd + d;
       *reinterpret_cast<__half2*>(cache + off) = hv;
     }
   }

@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kTcThreads2, TcCfg<NTILE>::kMinBlocks)
   } else {
     a.out = static_cast<__half*>(a0.out) + (size_t)tok0 * a0.H;
     a.pos = a0.pos + tok0;
+    if (a0.cidx) a.cidx = a0.cidx + tok0;
     if (a0.slots) a.slots = a0.slots + tok0;
     else a.slot0 = a0.slot0 + tok0;
   }

@@ -613,19 +613,23 @@ class DecodeEngine:
         return ptr(bufs.lora_t), ptr(b), self.lora_r
 
     # -- one step ----------------------------------------------------------------------
-    def run_layers(self, M: int, bufs: Optional[RowBuffers] = None, units: Optional[torch.Tensor] = None):
+    def run_layers(self, M: int, bufs: Optional[RowBuffers] = None, units: Optional[torch.Tensor] = None,
+                   serve=None):
         """All layers for rows [0, M) of `bufs` (default: the decode buffers): token ids in
         tok_in, positions in pos, cache slots in slots. `units` (prefill: a device copy of
         prefill_units for these rows) routes attention to the tensor-core prefill kernel,
-        which reads each sequence's keys once per 64 rows instead of once per row."""
+        which reads each sequence's keys once per 64 rows instead of once per row. `serve`
+        (serving.ServeRows) holds the rows' caches, the entries their keys go to and their
+        attention, where those are not the engine's own."""
         b = bufs if bufs is not None else self.dec
         cfg = self.cfg
         call("orch_embed_rows", ptr(b.tok_in), ptr(self.embed), F16 if self.embed.dtype == torch.float16 else F32,
              ptr(b.x), M, cfg.hidden_size, cfg.vocab_size, _stream())
         for li in range(len(self.layers)):
-            self.run_layer(li, M, b, units)
+            self.run_layer(li, M, b, units, serve)
 
-    def run_layer(self, li: int, M: int, bufs: Optional[RowBuffers] = None, units: Optional[torch.Tensor] = None):
+    def run_layer(self, li: int, M: int, bufs: Optional[RowBuffers] = None, units: Optional[torch.Tensor] = None,
+                  serve=None):
         """Layer `li` (LlamaLayer.forward, orchard/model.py:78-195) on the fp32 residual rows
         [0, M) of `bufs`.x in place, at the rows' positions and cache slots."""
         b = bufs if bufs is not None else self.dec
@@ -639,7 +643,9 @@ class DecodeEngine:
             attention_head_split(self._split_ops, self._comm, ctx, b, M)
             ffn_head_split(self._split_ops, self._comm, ctx, b, M)
             return
-        if L.tiled and "qkv" not in L.lora:
+        if serve is not None:
+            serve.append(self, li, M, b)
+        elif L.tiled and "qkv" not in L.lora:
             # RMSNorm fused in front of the projection (one launch for up to 8 rows)
             call("orch_q4t_rms_qkv_rope", ptr(L.tqkv), ptr(b.x), ptr(L.attn_norm), eps, ptr(b.xn), M, H, H, nh,
                  ptr(b.pos), ptr(b.slots), ptr(self.cos), ptr(self.sin), self.max_pos, ptr(b.q), ptr(kc), ptr(vc),
@@ -655,7 +661,9 @@ class DecodeEngine:
                 call("orch_q4_qkv_rope", ptr(L.wqkv), ptr(L.sqkv), ptr(b.xn), M, H, H, nh, ptr(b.pos),
                      ptr(b.slots), ptr(self.cos), ptr(self.sin), self.max_pos, ptr(b.q), ptr(kc), ptr(vc),
                      self.max_seq, self.num_slots, lt, lb, lr, s)
-        if units is not None:
+        if serve is not None:
+            serve.attend(self, li, M, b)
+        elif units is not None:
             call("orch_attention_prefill", ptr(b.q), ptr(kc), ptr(vc), ptr(units), units.shape[0],
                  ptr(b.attn), M, nh, hd, self.max_seq, self.num_slots, s)
         else:
@@ -690,10 +698,11 @@ class DecodeEngine:
         else:
             call("orch_q4_linear_resid", ptr(L.w2), ptr(L.s2), ptr(b.h), ptr(b.x), M, F, H, lt, lb, lr, s)
 
-    def run_head(self, M: int, temperature: float = 0.0):
+    def run_head(self, M: int, temperature: float = 0.0, controls=None):
         """Final RMSNorm, INT4 lm_head (fp32 logits) and the next token into tok_out: the
         argmax, or for temperature > 0 a draw from softmax(logits / T) with the row's
-        uniform in ``uniforms`` (orchard/model.py:244-252)."""
+        uniform in ``uniforms`` (orchard/model.py:244-252). ``controls``
+        (serving.RowControls) changes the logits before the choice."""
         b = self.dec
         cfg, s = self.cfg, _stream()
         H, V = cfg.hidden_size, cfg.vocab_size
@@ -709,6 +718,8 @@ class DecodeEngine:
         else:
             call("orch_gemm_q4_0_ex", ptr(self.lm_w), ptr(self.lm_s), ptr(b.xn), F16, ptr(b.logits), F32,
                  H, V, M, s)
+        if controls is not None:
+            controls.apply(b.logits, M, V)
         if temperature > 0:
             call("orch_sample_rows", ptr(b.logits), M, V, float(temperature), ptr(b.uniforms), ptr(b.tok_out), s)
         else:

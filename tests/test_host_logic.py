@@ -87,3 +87,14 @@ def test_prefill_units_cover_rows_in_runs():
     assert u[:, 0].tolist() == expect
     assert model.prefill_units([], []).shape == (0, 4)
     assert model.prefill_units(list(range(10)), [0] * 10, max_rows=4)[:, 1].tolist() == [4, 4, 2]
+
+
+def test_prefix_units_cover_the_rows():
+    """Units of orch_attention_prefix: every row once, in order, at most 128 rows each."""
+    from orchard_b200 import serving
+    for rows in (1, 127, 128, 129, 512, 700):
+        u = serving.prefix_units(rows, 3, 17)
+        assert u.dtype == np.int32 and (u[:, 2] == 3).all() and (u[:, 3] == 17).all()
+        assert u[:, 1].max() <= 128 and u[:, 1].min() >= 1
+        np.testing.assert_array_equal(np.concatenate([np.arange(a, a + n) for a, n, _, _ in u]), np.arange(rows))
+    assert serving.prefix_units(0, 0, 1).shape == (0, 4)
