@@ -12,8 +12,10 @@
 // vocabulary, requests the whole slice (16 logits per thread) before anything else, and while
 // those loads are in flight counts the row's history into a table of the slice in shared memory
 // (integer atomics: the result has no order). A slice is as small as keeps the grid within one
-// round of CTAs, so that few rows still use many SMs; wide batches take the largest slice, where
-// the history is read least often.
+// round of CTAs, so that few rows still use many SMs; wide batches take the largest slice, two
+// rounds of loads, where the history is read least often (128 rows x 131,072 with 4,095 ids of
+// history: 37 us, 42 us with slices of one round, 24 us with no control at all; sharing the
+// history over a cluster's tables took 93 us, its distributed-shared-memory atomics being slow).
 #include <algorithm>
 
 #include "orch_common.cuh"
@@ -24,9 +26,11 @@ namespace {
 
 constexpr int kLpThreads = 512;
 constexpr int kLpEach = 16;  // logits per thread at most
-constexpr int kLpMaxSlice = kLpThreads * kLpEach;
-// A table word of the slice. Packed: count (15 bits), seen (bit 15), bias entry + 1 (16 bits).
-// Histories or bias lists too long for that take two words: seen and count, and the bias entry.
+constexpr int kLpRounds = 2;  // of wide batches: a slice twice as large reads the history half as often
+constexpr int kLpMaxSlice = kLpThreads * kLpEach * kLpRounds;
+// A table word of the slice. Packed: occurrences that count (15 bits), seen before them (bit 15),
+// bias entry + 1 (16 bits). Histories or bias lists too long for that take two words:
+// occurrences and seen, and the bias entry.
 constexpr int kLpPackedHist = 32767, kLpPackedBias = 65534;
 
 struct LpArgs {
@@ -68,19 +72,22 @@ __global__ void __launch_bounds__(kLpThreads, 3) logits_process_kernel(const LpA
   const int mr = a.masks ? a.mask_rows[m] : -1;
   const T* in = static_cast<const T*>(a.in) + (size_t)m * a.ld + i0;
   LpVec<T, VEC> x[P];
+  auto load = [&](int r0) {  // this thread's logits of the round that begins at r0
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int i = (p * kLpThreads + tid) * VEC;
-    if (p < a.pieces) {
-      if (VEC == 1 || i + VEC <= n) {
-        if (i < n) x[p] = *reinterpret_cast<const LpVec<T, VEC>*>(in + i);
-      } else {
+    for (int p = 0; p < P; ++p) {
+      const int i = r0 + (p * kLpThreads + tid) * VEC;
+      if (p < a.pieces) {
+        if (VEC == 1 || i + VEC <= n) {
+          if (i < n) x[p] = *reinterpret_cast<const LpVec<T, VEC>*>(in + i);
+        } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (i + e < n) x[p].v[e] = in[i + e];
+          for (int e = 0; e < VEC; ++e)
+            if (i + e < n) x[p].v[e] = in[i + e];
+        }
       }
     }
-  }
+  };
+  load(0);
   if (hlen < 0 || hlen > a.hist_ld || b0 < 0 || b1 < b0 || b1 > a.num_bias || mr >= a.num_masks) {
     if (tid == 0) atomicOr(a.check, 16u);
     return;
@@ -109,8 +116,10 @@ __global__ void __launch_bounds__(kLpThreads, 3) logits_process_kernel(const LpA
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           if (v[u] < un) {
-            atomicOr(&lp_tab[v[u]], kSeen);
-            if (j0 + u * kLpThreads >= g0) atomicAdd(&lp_tab[v[u]], 1u);
+            if (j0 + u * kLpThreads >= g0)
+              atomicAdd(&lp_tab[v[u]], 1u);
+            else
+              atomicOr(&lp_tab[v[u]], kSeen);
           }
       }
     }
@@ -119,40 +128,62 @@ __global__ void __launch_bounds__(kLpThreads, 3) logits_process_kernel(const LpA
   const float rep = pen ? a.pen[3 * m] : 1.f, pres = pen ? a.pen[3 * m + 1] : 0.f, freq = pen ? a.pen[3 * m + 2] : 0.f;
   const uint32_t* mask = mr >= 0 ? a.masks + (size_t)mr * a.mask_words : nullptr;
   T* out = static_cast<T*>(a.out) + (size_t)m * a.ld + i0;
+  // one logit whose table words are not all zero
+  auto touch = [&](T v, uint32_t t, uint32_t b) {
+    float l = to_f32(v);
+    const uint32_t c = t & kCount;
+    if (t & (kSeen | kCount)) l = l > 0.f ? l / rep : l * rep;
+    if (c != 0u) l -= fmaf(freq, (float)c, pres);
+    if (b != 0u) l += a.bias_vals[b0 + (int)b - 1];
+    return from_f32<T>(l);
+  };
+  const int span = kLpThreads * VEC * a.pieces;  // logits of a round
+#pragma unroll 1
+  for (int r0 = 0; r0 < n; r0 += span) {
+    if (r0 > 0) load(r0);
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int i = (p * kLpThreads + tid) * VEC;
-    if (p >= a.pieces || i >= n) continue;
-    const uint32_t v0 = (uint32_t)(a.base + i0 + i);
-    // the mask bits of VEC ids from v0 on: a word, and the next one where they straddle
-    uint32_t ok = 0xffffffffu;
-    if (mask != nullptr) {
-      const uint32_t w = v0 >> 5, s = v0 & 31u, nw = (uint32_t)a.mask_words;
-      const uint32_t lo_w = w < nw ? mask[w] : 0u, hi_w = s + VEC > 32 && w + 1 < nw ? mask[w + 1] : 0u;
-      ok = __funnelshift_r(lo_w, hi_w, s);
-    }
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float l = to_f32(x[p].v[e]);
+    for (int p = 0; p < P; ++p) {
+      const int i = r0 + (p * kLpThreads + tid) * VEC;
+      if (p >= a.pieces || i >= n) continue;
       if (pen || bias) {
-        const uint32_t t = i + e < n ? lp_tab[i + e] : 0u;
-        if (t & kSeen) {
-          l = l > 0.f ? l / rep : l * rep;
-          const uint32_t c = t & kCount;
-          if (c != 0u) l -= fmaf(freq, (float)c, pres);
-        }
-        const uint32_t b = WIDE ? (bias && i + e < n ? btab[i + e] : 0u) : t >> 16;
-        if (b != 0u) l += a.bias_vals[b0 + (int)b - 1];
-      }
-      if (!(ok >> e & 1u)) l = -INFINITY;
-      x[p].v[e] = from_f32<T>(l);
-    }
-    if (VEC == 1 || i + VEC <= n) {
-      *reinterpret_cast<LpVec<T, VEC>*>(out + i) = x[p];
-    } else {
+        // most groups of VEC are untouched: their words are looked at together (the table ends
+        // on a multiple of VEC, its words past n are zero)
+        uint32_t t[VEC], any = 0u;
+        if (VEC >= 4) {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (i + e < n) out[i + e] = x[p].v[e];
+          for (int e = 0; e < VEC; e += 4) {
+            const uint4 w = *reinterpret_cast<const uint4*>(lp_tab + i + e);
+            t[e] = w.x, t[(e + 1) % VEC] = w.y, t[(e + 2) % VEC] = w.z, t[(e + 3) % VEC] = w.w;
+          }
+        } else {
+          t[0] = lp_tab[i];
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) any |= t[e] | (WIDE ? btab[i + e] : 0u);
+        if (any != 0u) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            const uint32_t b = WIDE ? btab[i + e] : t[e] >> 16;
+            if ((t[e] | b) != 0u) x[p].v[e] = touch(x[p].v[e], t[e], b);
+          }
+        }
+      }
+      if (mask != nullptr) {
+        // the mask bits of VEC ids from v0 on: a word, and the next one where they straddle
+        const uint32_t v0 = (uint32_t)(a.base + i0 + i), w = v0 >> 5, s = v0 & 31u, nw = (uint32_t)a.mask_words;
+        const uint32_t lo_w = w < nw ? mask[w] : 0u, hi_w = s + VEC > 32 && w + 1 < nw ? mask[w + 1] : 0u;
+        const uint32_t ok = __funnelshift_r(lo_w, hi_w, s);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (!(ok >> e & 1u)) x[p].v[e] = from_f32<T>(-INFINITY);
+      }
+      if (VEC == 1 || i + VEC <= n) {
+        *reinterpret_cast<LpVec<T, VEC>*>(out + i) = x[p];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (i + e < n) out[i + e] = x[p].v[e];
+      }
     }
   }
 }
@@ -169,7 +200,7 @@ int lp_launch(LpArgs a, cudaStream_t st) {
   const uint64_t round = 3 * (uint64_t)num_sms(), unit = kLpThreads * VEC;
   a.pieces = 1;
   while (a.pieces < kLpEach / VEC && (a.V + unit * a.pieces - 1) / (unit * a.pieces) * a.M > round) ++a.pieces;
-  a.slice = (int)unit * a.pieces;
+  a.slice = (int)unit * a.pieces * (a.pieces == kLpEach / VEC ? kLpRounds : 1);
   const dim3 grid((a.V + a.slice - 1) / a.slice, a.M), none(0, 0, 0);
   const size_t smem = a.hist || a.bias_ids ? (size_t)a.slice * 4 * (WIDE ? 2 : 1) : 0;
   ORCH_CUDA(launch_k(logits_process_kernel<T, VEC, WIDE>, grid, dim3(kLpThreads), smem, st, none, a));
