@@ -51,26 +51,44 @@ __device__ __forceinline__ int ap_at(int r, int c) {
   return r * HD + ((HD == 32 ? c ^ ((r >> 1) & 3) : c ^ (r & 7)) << 3);
 }
 
-// One tile: query rows i0 .. i0 + n - 1 of the (row, head of kv) pairs starting at row m0,
-// keys [j0, j1) of K/V rows at kb / vb; partials go to range `split`.
+// The keys of a tile: rows [j0, j1) at k / v, then rows [0, n2) at k2 / v2. srow, with own2 naming
+// the stretch it belongs to, takes the scores of the own entries (rows are the G heads).
+struct ApKeys {
+  const __half* k;
+  const __half* v;
+  int j0, j1;
+  const __half* k2;
+  const __half* v2;
+  int n2;
+  float* srow;
+  bool own2;
+};
+
+// One tile: query rows i0 .. i0 + n - 1 of the (row, head of kv) pairs starting at row m0, over
+// `keys`; partials go to range `split`. The statistics of the rows stay in shared memory.
 template <int HD, int WR>
-__device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, int kv, const __half* kb,
-                                        const __half* vb, int j0, int j1, int split, float* srow) {
+__device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, int kv, const ApKeys& keys, int split) {
   constexpr int WK = 4 / WR, TR = 16 * WR, TILE = kApKeys * HD, KT = kApKeys / 8 / WK;
   extern __shared__ __align__(16) uint8_t ap_smem[];
   __half* buf = reinterpret_cast<__half*>(ap_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int wrow = warp % WR, wkey = warp / WR;
-  const int nb = (j1 - j0 + kApKeys - 1) / kApKeys;
+  const int nb1 = (keys.j1 - keys.j0 + kApKeys - 1) / kApKeys, nb = nb1 + (keys.n2 + kApKeys - 1) / kApKeys;
+  // block b's first row and the end of its stretch
+  auto first = [&](int b) { return b < nb1 ? keys.j0 + b * kApKeys : (b - nb1) * kApKeys; };
+  auto end = [&](int b) { return b < nb1 ? keys.j1 : keys.n2; };
 
   auto issue = [&](int b) {
+    const __half* kb = b < nb1 ? keys.k : keys.k2;
+    const __half* vb = b < nb1 ? keys.v : keys.v2;
+    const int k0 = first(b), k1 = end(b);
     __half* kd = buf + (b & 1) * 2 * TILE;
     __half* vd = kd + TILE;
     constexpr int CPR = HD / 8;  // 16-byte pieces per row
 #pragma unroll
     for (int j = 0; j < kApKeys * CPR / 128; ++j) {
-      const int i = tid + 128 * j, r = i / CPR, c8 = i % CPR, key = j0 + b * kApKeys + r;
-      const bool ok = key < j1;
+      const int i = tid + 128 * j, r = i / CPR, c8 = i % CPR, key = k0 + r;
+      const bool ok = key < k1;
       const size_t off = ok ? (size_t)key * HD + c8 * 8 : 0;
       ap_cp16(kd + ap_at<HD>(r, c8), kb + off, ok);
       ap_cp16(vd + ap_at<HD>(r, c8), vb + off, ok);
@@ -134,25 +152,26 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
       }
     }
     float bm0 = -INFINITY, bm1 = -INFINITY;
+    const int k0 = first(b), k1 = end(b);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const bool ok = j0 + b * kApKeys + 8 * (kt0 + t) + 2 * c + e < j1;
+        const bool ok = k0 + 8 * (kt0 + t) + 2 * c + e < k1;
         sc[t][e] = ok ? sc[t][e] * scale : -INFINITY;
         sc[t][2 + e] = ok ? sc[t][2 + e] * scale : -INFINITY;
         bm0 = fmaxf(bm0, sc[t][e]);
         bm1 = fmaxf(bm1, sc[t][2 + e]);
       }
-    if (srow != nullptr) {  // the own entries' scores, for their weights (rows are the G heads)
+    if (keys.srow != nullptr && (b >= nb1) == keys.own2) {  // the own entries' scores, for their weights
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int key = j0 + b * kApKeys + 8 * (kt0 + t) + 2 * c + e;
-          if (key < j1) {
-            if (qr < n) srow[(size_t)(i0 + qr) * a.lds + key] = sc[t][e];
-            if (qr + 8 < n) srow[(size_t)(i0 + qr + 8) * a.lds + key] = sc[t][2 + e];
+          const int key = k0 + 8 * (kt0 + t) + 2 * c + e;
+          if (key < k1) {
+            if (qr < n) keys.srow[(size_t)(i0 + qr) * a.lds + key] = sc[t][e];
+            if (qr + 8 < n) keys.srow[(size_t)(i0 + qr + 8) * a.lds + key] = sc[t][2 + e];
           }
         }
     }
@@ -257,17 +276,37 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
       if (d == 0) a.stat[mh * S + split] = make_float2(mx, l);
     }
   }
+  if (a.direct && keys.srow != nullptr) {  // the only row: its own entries' weights (n is G here)
+    __syncthreads();  // scores written; O no longer needed
+    float2* tot = reinterpret_cast<float2*>(ap_smem);
+    if (tid < n) {
+      float mx = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) mx = fmaxf(mx, ss[w * TR + tid].x);
+#pragma unroll
+      for (int w = 0; w < WK; ++w) l += ss[w * TR + tid].x == -INFINITY ? ss[w * TR + tid].y : ap_exp2(ss[w * TR + tid].x - mx) * ss[w * TR + tid].y;
+      tot[tid] = make_float2(mx == -INFINITY ? 0.f : mx - kApShift, l == 0.f ? 0.f : 1.0f / l);
+    }
+    __syncthreads();
+    const int len = keys.own2 ? keys.n2 : keys.j1;
+    float* mass = a.mass + ((size_t)(a.slots ? a.slots[m0] : m0) * a.nkv + kv) * a.max_seq;
+    for (int e = tid; e < len; e += 128) {
+      float w = 0.f;
+      for (int h = 0; h < n; ++h) w = fmaf(ap_exp2(keys.srow[(size_t)h * a.lds + e] - tot[h].x), tot[h].y, w);
+      mass[e] = e == len - 1 ? w : mass[e] + w;
+    }
+  }
 }
 
 template <int HD>
-__device__ __forceinline__ void ap_tile_wr(int wr, const ApArgs& a, int m0, int i0, int n, int kv, const __half* kb,
-                                           const __half* vb, int j0, int j1, int split, float* srow) {
+__device__ __forceinline__ void ap_tile_wr(int wr, const ApArgs& a, int m0, int i0, int n, int kv, const ApKeys& keys,
+                                           int split) {
   if (wr == 1)
-    ap_tile<HD, 1>(a, m0, i0, n, kv, kb, vb, j0, j1, split, srow);
+    ap_tile<HD, 1>(a, m0, i0, n, kv, keys, split);
   else if (wr == 2)
-    ap_tile<HD, 2>(a, m0, i0, n, kv, kb, vb, j0, j1, split, srow);
+    ap_tile<HD, 2>(a, m0, i0, n, kv, keys, split);
   else
-    ap_tile<HD, 4>(a, m0, i0, n, kv, kb, vb, j0, j1, split, srow);
+    ap_tile<HD, 4>(a, m0, i0, n, kv, keys, split);
 }
 
 template <int HD>
@@ -289,7 +328,8 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
     if (j0 >= j1) return;
     const size_t base = ((size_t)u.z * a.nkv + kv) * a.prefix_cap * HD;
-    ap_tile_wr<HD>(a.wr_p, a, u.x, i0, n, kv, a.kp + base, a.vp + base, j0, j1, split, nullptr);
+    ap_tile_wr<HD>(a.wr_p, a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
+                   split);
     return;
   }
   b -= a.blocks_p;  // a range of one row's own entries for the G heads of a K/V head
@@ -305,16 +345,11 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
   }
   const int tr = 16 * a.wr_o, i0 = tile * tr, n = min(tr, a.G - i0);
   const int per = ap_range(len, a.S_o), j0 = split * per, j1 = min(len, j0 + per);
-  if (j0 >= j1) {
-    if (a.direct && len == 0) {  // nothing to attend to
-      for (int i = threadIdx.x; i < n * HD; i += 128)
-        a.out[((size_t)m * a.nh + kv * a.G + i0) * HD + i] = __float2half_rn(0.f);
-    }
-    return;
-  }
+  if (j0 >= j1) return;
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
   float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, a.kc + base, a.vc + base, j0, j1, a.S_p + split, srow);
+  ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
+                 a.S_p + split);
 }
 
 template <int HD>
@@ -328,18 +363,18 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
   if (a.tc && blockIdx.x == 0) pdl_wait();
 }
 
-// Ranges of row m that hold keys: prefix ranges 0 .. np - 1, own ranges S_p .. S_p + no - 1.
-// False when the row or its unit was rejected. (Called by whole warps.)
-__device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int& len, int& np, int& no) {
+// The prefix of row m: its slot and length (0: none). False when the row's unit was rejected or
+// the row is in two. (Called by whole warps.)
+__device__ __forceinline__ bool ap_row_prefix(const ApArgs& a, int m, int& pslot, int& plen) {
   const int lane = threadIdx.x & 31;
-  int plen = 0, bad = 0, in = 0;
+  int bad = 0, in = 0, z = 0, w = 0;
   for (int u0 = 0; u0 < a.num_units; u0 += 32) {
     const int i = u0 + lane;
     if (i < a.num_units) {
       const int4 u = a.units[i];
       if (m >= u.x && (long long)m < (long long)u.x + u.y) {
         if (ap_unit_ok(a, u)) {
-          plen = max(plen, u.w);
+          z = u.z, w = u.w;
           ++in;
         } else {
           bad = 1;
@@ -347,14 +382,49 @@ __device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int
       }
     }
   }
-  const bool ok = ap_row(a, m, slot, len);
-  plen = __reduce_max_sync(0xffffffffu, plen);
   in = (int)__reduce_add_sync(0xffffffffu, (unsigned)in);
-  if (in > 1 && lane == 0) atomicOr(a.check, 2u);  // in two units
-  if (__any_sync(0xffffffffu, bad) || !ok || in > 1) return false;
+  if (in > 1 && lane == 0) atomicOr(a.check, 2u);
+  pslot = (int)__reduce_add_sync(0xffffffffu, (unsigned)z);  // one lane's at most, when in <= 1
+  plen = (int)__reduce_add_sync(0xffffffffu, (unsigned)w);
+  return !__any_sync(0xffffffffu, bad) && in <= 1;
+}
+
+// Ranges of row m that hold keys: prefix ranges 0 .. np - 1, own ranges S_p .. S_p + no - 1.
+// False when the row or its unit was rejected. (Called by whole warps.)
+__device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int& len, int& np, int& no) {
+  int pslot, plen;
+  const bool ok = ap_row(a, m, slot, len);
+  if (!ap_row_prefix(a, m, pslot, plen) || !ok) return false;
   np = plen > 0 ? (plen + ap_range(plen, a.S_p, a.blk_p) - 1) / ap_range(plen, a.S_p, a.blk_p) : 0;
   no = len > 0 ? (len + ap_range(len, a.S_o) - 1) / ap_range(len, a.S_o) : 0;
   return true;
+}
+
+// Few rows and few keys: a CTA takes one row's G heads of a K/V head through the prefix and the
+// own entries and writes the output itself, in one launch.
+template <int HD>
+__global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int tile = blockIdx.x % a.tiles_o, b = blockIdx.x / a.tiles_o, kv = b % a.nkv, m = b / a.nkv;
+  if (blockIdx.x == 0)  // units are reported once, whether or not a row is in them
+    for (int i = threadIdx.x; i < a.num_units; i += 128) {
+      const int4 u = a.units[i];
+      if (!ap_unit_ok(a, u)) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
+    }
+  int slot, len, pslot, plen;
+  const bool row = ap_row(a, m, slot, len);
+  if (!row && threadIdx.x == 0) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
+  if (!ap_row_prefix(a, m, pslot, plen) || !row) return;
+  const int tr = 16 * a.wr_o, i0 = tile * tr, n = min(tr, a.G - i0);
+  if (plen + len == 0) {  // nothing to attend to
+    for (int i = threadIdx.x; i < n * HD; i += 128)
+      a.out[((size_t)m * a.nh + kv * a.G + i0) * HD + i] = __float2half_rn(0.f);
+    return;
+  }
+  const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD, pb = ((size_t)pslot * a.nkv + kv) * a.prefix_cap * HD;
+  float* srow = a.mass && len > 0 ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
+  ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
 }
 
 template <int V>
@@ -521,6 +591,7 @@ struct ApPlan {
   size_t bytes() const { return (acc_floats + stat_floats + score_floats) * sizeof(float); }
 };
 
+constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V heads, keys of a row: one launch
 constexpr int kApTcFrom = 32;  // query rows of a unit above which its prefix takes the tcgen05 tiles
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
@@ -560,7 +631,12 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
     p.S_p = ranges(items, max_prefix, 64 * p.wr_p + 64);
   }
   p.S_o = ranges((size_t)M * nkv * p.tiles_o, max_own, 64);  // at least one: rows are checked there
-  p.direct = p.S_p == 0 && p.S_o == 1 && !track;
+  // Few CTAs with little to read: splitting would cost a second launch and more than it saves (2 x
+  // 2 heads of 32 keys: 3.2 us in one launch, 4.9 in two; one row of 32 heads x 577 keys, tracked:
+  // 15.9 and 9.7). Weights only for a single row: rows that share a slot need an order.
+  p.direct = (size_t)M * nkv <= kApDirectPairs && (some ? max_prefix : 0) + (uint64_t)max_own <= kApDirectKeys &&
+             (!track || (M == 1 && p.tiles_o == 1));
+  if (p.direct) p.tc = 0;
   const size_t mh = (size_t)M * nh, S = p.S_p + p.S_o;
   p.acc_floats = p.direct ? 0 : mh * S * hd;
   p.stat_floats = p.direct ? 0 : (mh * S * 2 + 3) / 4 * 4;
@@ -578,6 +654,7 @@ int ap_launch(ApArgs a, cudaStream_t st) {
   const int dev = device_index();
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
     ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_done[dev] = true;
   }
   const dim3 none(0, 0, 0);
@@ -586,17 +663,20 @@ int ap_launch(ApArgs a, cudaStream_t st) {
     if (rc != ORCH_OK) return rc;
     a.blocks_p = 0;
   }
+  if (a.direct) {
+    ORCH_CUDA(launch_k_serial(attn_prefix_row_kernel<HD>, dim3((unsigned)(a.M * a.nkv * a.tiles_o)), dim3(128), smem, st,
+                              none, a));
+    return check_launch("attention_prefix");
+  }
   const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
   ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
-  if (!a.direct) {
-    const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
-    const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
-    const size_t jb = (size_t)blocks_out + (size_t)a.M * a.nkv * chunks;
-    if (jb > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
-    ORCH_CUDA(launch_k(attn_prefix_join_kernel<HD>, dim3((unsigned)jb), dim3(128), 0, st, none, a, blocks_out,
-                       std::max(chunks, 1)));
-  }
+  const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
+  const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
+  const size_t jb = (size_t)blocks_out + (size_t)a.M * a.nkv * chunks;
+  if (jb > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
+  ORCH_CUDA(launch_k(attn_prefix_join_kernel<HD>, dim3((unsigned)jb), dim3(128), 0, st, none, a, blocks_out,
+                     std::max(chunks, 1)));
   return check_launch("attention_prefix");
 }
 

@@ -33,7 +33,7 @@ struct ApArgs {
   int blk_p;             // keys that a range of a prefix is a multiple of
   int tc;                // the prefix part runs in its own kernel (attention_prefix_tc.cu)
   int blocks_p;          // CTAs of the prefix part (the first ones of the grid)
-  int direct;            // one range in all: the output is written by the attention kernel
+  int direct;            // few rows and keys: one launch, the output written by the attention kernel
   float* acc;            // [M * nh][S][HD]
   float2* stat;          // [M * nh][S]: (max, sum), in powers of two
   float* scores;         // [M * nh][lds], with mass only

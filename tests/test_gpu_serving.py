@@ -176,13 +176,15 @@ def test_infinite_and_nan_keys_inside_the_lengths():
     assert np.all(np.abs(out[1, 1] - want[1, 1]) <= bound[1, 1])
 
 
-@pytest.mark.parametrize("hd,nh,nkv,plen,lens", [(128, 4, 4, 0, [577]), (64, 8, 2, 100, [1, 2, 63, 64, 65, 0]),
+@pytest.mark.parametrize("hd,nh,nkv,plen,lens", [(128, 4, 4, 0, [577]), (64, 60, 3, 100, [66]), (32, 5, 5, 77, [0]),
+                                                 (128, 32, 32, 0, [190]), (64, 70, 1, 10, [40]), (128, 6, 2, 130, [1]), (64, 8, 2, 100, [1, 2, 63, 64, 65, 0]),
                                                  (32, 6, 1, 30, [1500, 3]), (128, 40, 2, 0, [1, 1030])])
 def test_tracked_weights(hd, nh, nkv, plen, lens):
     M = len(lens)
     units = [(0, M, 0, plen)] if plen else []
-    host = case(20 + M, hd, nh, nkv, units, lens, 1500, nslots=M + 1, pcap=max(plen, 1))
-    mass = rng(2, M).random((M + 1, nkv, 1500), dtype=np.float32)
+    cap = max(1500 if M > 1 else 0, max(lens), 1)
+    host = case(20 + M, hd, nh, nkv, units, lens, cap, nslots=M + 1, pcap=max(plen, 1))
+    mass = rng(2, M).random((M + 1, nkv, cap), dtype=np.float32)
     check_attention(host, mass)
 
 
@@ -230,22 +232,25 @@ def test_prefix_attention_repeats_and_serves_a_captured_graph():
     check_attention((q, kp, vp, units, kc, vc, lens, slots), got=out)
 
 
-def test_prefix_attention_skips_bad_rows_and_units():
+@pytest.mark.parametrize("track,cap", [(True, 10), (False, 10), (False, 700)])
+def test_prefix_attention_skips_bad_rows_and_units(track, cap):
     q, kp, vp, units, kc, vc, lens, slots = case(50, 64, 4, 2, [(0, 2, 0, 30), (2, 2, 0, 30), (4, 2, 0, 30)], [3, 4, 5, 6, 7, 8],
-                                                10, nslots=6, pcap=30, poison=False)
-    good = attention(*[D(x) for x in (q, kp, vp, units, kc, vc, lens, slots)]).cpu()
-    mass = torch.zeros((6, 2, 10), device="cuda")
+                                                cap, nslots=6, pcap=30, poison=False)
+    mass = torch.zeros((6, 2, cap), device="cuda")
 
     def go(u=units, n=lens, s=slots):
         mass.zero_()
-        return attention(D(q), D(kp), D(vp), D(u), D(kc), D(vc), D(n), D(s), mass).cpu()
+        return attention(D(q), D(kp), D(vp), D(u), D(kc), D(vc), D(n), D(s), mass if track else None).cpu()
 
-    for bad in (-1, 11, 2 ** 31 - 1):
+    good = go()
+    assert flags() == 0
+
+    for bad in (-1, cap + 1, 2 ** 31 - 1):
         n = lens.copy()
         n[1] = bad
         o = go(n=n)
         assert flags() == 2 and (o[1] == 7).all() and torch.equal(o[[0, 2, 3, 4, 5]], good[[0, 2, 3, 4, 5]])
-        assert not mass[slots[1]].any() and mass[slots[0]].any()
+        assert not mass[slots[1]].any() and bool(mass[slots[0]].any()) == track
     for bad in (-1, 6, 2 ** 31 - 1):
         s = slots.copy()
         s[4] = bad
@@ -261,6 +266,10 @@ def test_prefix_attention_skips_bad_rows_and_units():
     u[2] = (4, 3, 0, 30)  # one row more than there are
     o = go(u=u)
     assert flags() == 2 and (o[4:] == 7).all() and torch.equal(o[:4], good[:4])
+    u = units.copy()
+    u[1] = (1, 3, 0, 30)  # row 1 in two units
+    o = go(u=u)
+    assert flags() == 2 and (o[1] == 7).all() and (o[0] != 7).any()
 
 
 def test_prefix_attention_beyond_32_bit_offsets():

@@ -1,8 +1,13 @@
-"""Refusals of the serving operators: argument checks that run before any device work (no GPU)."""
+"""Refusals of the serving operators: argument checks that run before any device work. They run
+where there is no GPU only: the pointers are stand-ins, and a call that were accepted by mistake
+must not reach a device."""
 
 import pytest
+import torch
 
 from orchard_b200 import _lib
+
+pytestmark = pytest.mark.skipif(torch.cuda.is_available(), reason="the pointers stand for nothing: no GPU may see them")
 
 P = 4096  # stands for a 16-byte aligned device pointer: never read, the checks come first
 
@@ -34,7 +39,7 @@ def logits(**kw):
     (dict(hd=48), b"head_dim"), (dict(hd=256), b"head_dim"), (dict(mo=9), b"max_own"), (dict(ns=0), b"cache shape"),
     (dict(cap=0, mo=0), b"cache shape"), (dict(cap=2 ** 30), b"cache shape"), (dict(mp=9), b"max_prefix"),
     (dict(np_=0), b"prefix shape"), (dict(q=P + 2), b"aligned"), (dict(units=P + 4), b"aligned"), (dict(ws=P + 8, wb=1 << 30), b"aligned"),
-    (dict(ws=None), b"workspace"), (dict(ws=P, wb=16), b"workspace")])
+    (dict(ws=None, mo=4000, cap=4000), b"workspace"), (dict(ws=P, wb=16, mo=4000, cap=4000), b"workspace")])
 def test_attention_refusals(kw, word):
     assert attention(**kw) == 1 and word in _lib.lib().orch_last_error()
 
@@ -66,5 +71,6 @@ def test_unsupported_shapes_and_empty_calls():
 def test_workspace_size():
     f = _lib.lib().orch_attention_prefix_workspace_bytes
     assert f(0, 4, 4, 64, 1, 100, 100, 0) == 0 and f(1, 4, 3, 64, 1, 100, 100, 0) == 0
+    assert f(1, 2, 2, 32, 1, 24, 8, 0) == 0  # one launch, nothing to join
     assert f(64, 32, 32, 128, 1, 4096, 640, 0) > 64 * 32 * 128 * 4
     assert f(64, 32, 32, 128, 1, 4096, 640, 1) >= f(64, 32, 32, 128, 1, 4096, 640, 0) + 64 * 32 * 640 * 4
