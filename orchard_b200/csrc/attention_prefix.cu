@@ -22,6 +22,7 @@
 // (max, sum, O) meet in shared memory at the end, so few rows still keep every warp at work.
 // K and V blocks of 64 keys are copied by cp.async into a double buffer.
 #include <algorithm>
+#include <cmath>
 
 #include "attention_prefix.cuh"
 
@@ -345,7 +346,12 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
   }
   const int tr = 16 * a.wr_o, i0 = tile * tr, n = min(tr, a.G - i0);
   const int per = ap_range(len, a.S_o), j0 = split * per, j1 = min(len, j0 + per);
-  if (j0 >= j1) return;
+  if (j0 >= j1) {
+    if (a.direct && len == 0)  // nothing to attend to
+      for (int i = threadIdx.x; i < n * HD; i += 128)
+        a.out[((size_t)m * a.nh + kv * a.G + i0) * HD + i] = __float2half_rn(0.f);
+    return;
+  }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
   float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
   ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
@@ -450,7 +456,7 @@ __device__ __forceinline__ float2 ap_total(const ApArgs& a, size_t mh, int np, i
 // Joins the ranges: one warp per (row, head) for the output; with mass, further CTAs each
 // take kMassEntries entries of one (row, K/V head).
 constexpr int kMassEntries = 512;
-constexpr int kMassHeads = 32;  // heads whose totals are held at once
+constexpr int kMassHeads = 4;  // heads of a K/V head taken at once
 
 template <int HD>
 __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, int blocks_out, int chunks) {
@@ -463,7 +469,7 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
     if (mh >= a.M * a.nh) return;
     // The first ranges' records are requested before it is known which of them hold keys, so
     // that the kernel waits on L2 once; what a range without keys left there is not used.
-    constexpr int V = HD / 32, U = 8;  // values per lane, ranges requested ahead
+    constexpr int V = HD / 32, U = 12;  // values per lane, ranges requested ahead
     const float* ac = a.acc + (size_t)mh * S * HD + lane * V;
     const float2* st = a.stat + (size_t)mh * S;
     ApVec<V> pre[U];
@@ -527,6 +533,22 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
   const int kv = b % a.nkv, m = b / a.nkv;
   int slot, len, np, no;
   if (!ap_ranges(a, m, slot, len, np, no)) return;
+  constexpr int E = kMassEntries / 128;  // entries per thread
+  const int e0 = chunk * kMassEntries;
+  float* mass = a.mass + ((size_t)slot * a.nkv + kv) * a.max_seq;
+  // the scores of kMassHeads heads of row r, requested before their totals are known
+  float sv[kMassHeads][E];
+  auto fetch = [&](int r, int h0) {
+    const float* sr = a.scores + ((size_t)r * a.nh + kv * a.G + h0) * a.lds;
+#pragma unroll
+    for (int j = 0; j < kMassHeads; ++j)
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int e = e0 + threadIdx.x + 128 * i;
+        sv[j][i] = j < a.G - h0 && e < len ? sr[(size_t)j * a.lds + e] : -INFINITY;
+      }
+  };
+  fetch(m, 0);
   __shared__ int any;
   __shared__ float2 tots[kMassHeads];
   if (threadIdx.x == 0) any = 0;
@@ -544,40 +566,35 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
       if (ap_ranges(a, r, s2, l2, p2, o2)) return;
     }
   }
-  float* mass = a.mass + ((size_t)slot * a.nkv + kv) * a.max_seq;
   const int last = (any & 2) ? a.M - 1 : m;
   for (int r = m; r <= last; ++r) {
-    if ((a.slots ? a.slots[r] : r) != slot) continue;
-    int s2;
-    if (r != m && !ap_ranges(a, r, s2, len, np, no)) continue;
-    const int e0 = chunk * kMassEntries;
-    if (e0 >= len) continue;
-    float w[kMassEntries / 128];
+    if (r != m) {
+      int s2;
+      if ((a.slots ? a.slots[r] : r) != slot || !ap_ranges(a, r, s2, len, np, no) || e0 >= len) continue;
+      fetch(r, 0);
+    } else if (e0 >= len) {
+      continue;
+    }
+    float w[E];
 #pragma unroll
-    for (int i = 0; i < kMassEntries / 128; ++i) w[i] = 0.f;
+    for (int i = 0; i < E; ++i) w[i] = 0.f;
     for (int h0 = 0; h0 < a.G; h0 += kMassHeads) {
       const int hs = min(kMassHeads, a.G - h0);
+      if (h0 > 0) fetch(r, h0);
       __syncthreads();  // the totals of the heads before are done with
       for (int j = warp; j < hs; j += 4) {  // the heads' totals, a warp each
         const float2 tot = ap_total(a, (size_t)r * a.nh + kv * a.G + h0 + j, np, no);
         if (lane == 0) tots[j] = make_float2(tot.x == -INFINITY ? 0.f : tot.x - kApShift, tot.y == 0.f ? 0.f : 1.0f / tot.y);
       }
       __syncthreads();
-      for (int j = 0; j < hs; ++j) {
-        const float2 tot = tots[j];
-        const float* sr = a.scores + ((size_t)r * a.nh + kv * a.G + h0 + j) * a.lds;
-        float sv[kMassEntries / 128];
 #pragma unroll
-        for (int i = 0; i < kMassEntries / 128; ++i) {
-          const int e = e0 + threadIdx.x + 128 * i;
-          sv[i] = e < len ? sr[e] : -INFINITY;
-        }
+      for (int j = 0; j < kMassHeads; ++j)
+        if (j < hs)
 #pragma unroll
-        for (int i = 0; i < kMassEntries / 128; ++i) w[i] = fmaf(ap_exp2(sv[i] - tot.x), tot.y, w[i]);
-      }
+          for (int i = 0; i < E; ++i) w[i] = fmaf(ap_exp2(sv[j][i] - tots[j].x), tots[j].y, w[i]);
     }
 #pragma unroll
-    for (int i = 0; i < kMassEntries / 128; ++i) {
+    for (int i = 0; i < E; ++i) {
       const int e = e0 + threadIdx.x + 128 * i;
       if (e < len) mass[e] = e == len - 1 ? w[i] : mass[e] + w[i];
     }
@@ -586,7 +603,7 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
 
 // How a call is cut: rows per tile, key ranges, workspace. The same for the size query.
 struct ApPlan {
-  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, blk_p, tr_p, tc, direct, lds;
+  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, blk_p, tr_p, tc, row, direct, lds;
   size_t acc_floats, stat_floats, score_floats;
   size_t bytes() const { return (acc_floats + stat_floats + score_floats) * sizeof(float); }
 };
@@ -620,12 +637,18 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   const size_t items = nkv * likely;
   p.S_p = 0;
   if (p.tc) {
-    // one CTA per SM: the cut whose rounds cost least, a range's start and end counted as two blocks
-    const size_t blocks = (max_prefix + kApTcKeys - 1) / kApTcKeys, sms = num_sms();
-    size_t best = 0;
-    for (size_t s = 1; s <= std::min<size_t>(blocks, sms); ++s) {
-      const size_t cost = (items * s + sms - 1) / sms * ((blocks + s - 1) / s + 2);
-      if (p.S_p == 0 || cost < best) p.S_p = (int)s, best = cost;
+    // One CTA per SM, and the own entries' CTAs run on the other SMs meanwhile: the cut whose
+    // estimated time is least, in us. A block takes ~1.5 (128 rows) or ~2.7 (256), a range's start
+    // and end ~5, and an SM gets through ~35 KB of own entries per us (they are taken to be half as
+    // long as they may be).
+    const double sms = num_sms(), blocks = (max_prefix + kApTcKeys - 1) / kApTcKeys;
+    const double own = (double)M * nkv * max_own * 2.0 * hd / 35e3, block = p.tr_p > kApTcRows ? 2.7 : 1.5;
+    double best = 0;
+    for (int c = 1; c <= (int)std::min(blocks, sms); ++c) {
+      const double n = (double)items * c, run = std::ceil(blocks / c) * block + 5.0;
+      const double tc = std::ceil(n / sms) * run, beside = n < sms ? (sms - n) * tc : 0.0;
+      const double cost = tc + std::max(0.0, own - beside) / sms;
+      if (p.S_p == 0 || cost < best) p.S_p = c, best = cost;
     }
   } else if (some) {
     p.S_p = ranges(items, max_prefix, 64 * p.wr_p + 64);
@@ -634,9 +657,11 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   // Few CTAs with little to read: splitting would cost a second launch and more than it saves (2 x
   // 2 heads of 32 keys: 3.2 us in one launch, 4.9 in two; one row of 32 heads x 577 keys, tracked:
   // 15.9 and 9.7). Weights only for a single row: rows that share a slot need an order.
-  p.direct = (size_t)M * nkv <= kApDirectPairs && (some ? max_prefix : 0) + (uint64_t)max_own <= kApDirectKeys &&
+  p.row = (size_t)M * nkv <= kApDirectPairs && (some ? max_prefix : 0) + (uint64_t)max_own <= kApDirectKeys &&
              (!track || (M == 1 && p.tiles_o == 1));
-  if (p.direct) p.tc = 0;
+  if (p.row) p.tc = 0;
+  // one range per row in all: nothing to join either
+  p.direct = p.row || (!some && p.S_o == 1 && !track);
   const size_t mh = (size_t)M * nh, S = p.S_p + p.S_o;
   p.acc_floats = p.direct ? 0 : mh * S * hd;
   p.stat_floats = p.direct ? 0 : (mh * S * 2 + 3) / 4 * 4;
@@ -663,7 +688,7 @@ int ap_launch(ApArgs a, cudaStream_t st) {
     if (rc != ORCH_OK) return rc;
     a.blocks_p = 0;
   }
-  if (a.direct) {
+  if (a.row) {
     ORCH_CUDA(launch_k_serial(attn_prefix_row_kernel<HD>, dim3((unsigned)(a.M * a.nkv * a.tiles_o)), dim3(128), smem, st,
                               none, a));
     return check_launch("attention_prefix");
@@ -671,6 +696,7 @@ int ap_launch(ApArgs a, cudaStream_t st) {
   const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
   ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
+  if (a.direct) return check_launch("attention_prefix");
   const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
   const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
   const size_t jb = (size_t)blocks_out + (size_t)a.M * a.nkv * chunks;
@@ -763,6 +789,7 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   if (blocks_p > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many units for one launch");
   a.blocks_p = (int)blocks_p;
   a.direct = p.direct;
+  a.row = p.row;
   a.acc = static_cast<float*>(workspace);
   a.stat = reinterpret_cast<float2*>(a.acc + p.acc_floats);
   a.scores = a.acc + p.acc_floats + p.stat_floats;

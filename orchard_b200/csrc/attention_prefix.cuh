@@ -33,7 +33,8 @@ struct ApArgs {
   int blk_p;             // keys that a range of a prefix is a multiple of
   int tc;                // the prefix part runs in its own kernel (attention_prefix_tc.cu)
   int blocks_p;          // CTAs of the prefix part (the first ones of the grid)
-  int direct;            // few rows and keys: one launch, the output written by the attention kernel
+  int row;               // few rows and keys: a CTA per row and K/V head takes all of them
+  int direct;            // the output is written by the attention kernel: nothing to join
   float* acc;            // [M * nh][S][HD]
   float2* stat;          // [M * nh][S]: (max, sum), in powers of two
   float* scores;         // [M * nh][lds], with mass only

@@ -48,7 +48,8 @@ struct PtCfg {
   static constexpr int OffStat = Rows * OP * 4;
   static constexpr int Bytes = (OffStat + 2 * kApTcRows * 8 > OffBar ? OffStat + 2 * kApTcRows * 8 : OffBar);
   static constexpr int OffRef = Bytes + 256;  // a row's ref (floats), behind the barriers
-  static constexpr int Smem = OffRef + kApTcRows * 4;
+  static constexpr int OffRec = OffRef + kApTcRows * 4;  // a row's number among all (row, head) pairs
+  static constexpr int Smem = OffRec + Rows * 4;
   static constexpr uint32_t ColP = PAIR ? 0 : 256, StepP = PAIR ? 128 : 64;    // weights of group g
   static constexpr uint32_t ColO = PAIR ? 256 : 384, StepO = PAIR ? HD : 0;  // its accumulator
 };
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     __syncwarp();
   } else {
+    if (tid < n) reinterpret_cast<int*>(sm + C::OffRec)[tid] = (u.x + (i0 + tid) / a.G) * a.nh + kv * a.G + (i0 + tid) % a.G;
     // Q rows into their swizzled places: 16-byte piece c of a 128-byte row r at c ^ (r & 7).
     // Up to eight pieces per thread are requested before the first is stored.
     constexpr int Pieces = C::Rows * (HD / 8) / 256, Batch = Pieces < 8 ? Pieces : 8;
@@ -401,12 +403,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const int S = a.S_p + a.S_o;
     // the other kernels' records hold weights as 2^kApShift e^(s - max): the same scale here
     const float g = exp2f(kApShift - kPtShift);
+    const int* recs = reinterpret_cast<const int*>(sm + C::OffRec);
 #pragma unroll 4
     for (int i = tid; i < (good ? n * LPR : 0); i += 256) {
       const int r = i / LPR, d = (i % LPR) * 4;
-      const size_t rec = ((size_t)(u.x + (i0 + r) / a.G) * a.nh + kv * a.G + (i0 + r) % a.G) * S + split;
       const float4 ov = *reinterpret_cast<const float4*>(os + r * C::OP + d);
-      *reinterpret_cast<float4*>(a.acc + rec * HD + d) = make_float4(ov.x * g, ov.y * g, ov.z * g, ov.w * g);
+      *reinterpret_cast<float4*>(a.acc + ((size_t)recs[r] * S + split) * HD + d) = make_float4(ov.x * g, ov.y * g, ov.z * g, ov.w * g);
     }
     if (good && tid < n) {
       const int r = tid;
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         st.y = (st.x == at ? st.y : st.y * ap_exp2(st.x - at)) + (s1.x == at ? s1.y : s1.y * ap_exp2(s1.x - at));
         st.x = at;
       }
-      a.stat[((size_t)(u.x + (i0 + r) / a.G) * a.nh + kv * a.G + (i0 + r) % a.G) * S + split] = make_float2(st.x, st.y * g);
+      a.stat[(size_t)recs[r] * S + split] = make_float2(st.x, st.y * g);
     }
   }
   tc_fence_before();
