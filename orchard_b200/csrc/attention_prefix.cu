@@ -79,20 +79,23 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
   auto first = [&](int b) { return b < nb1 ? keys.j0 + b * kApKeys : (b - nb1) * kApKeys; };
   auto end = [&](int b) { return b < nb1 ? keys.j1 : keys.n2; };
 
+  // A thread copies piece c8 of rows r0, r0 + RS, ..: RS keeps the permutation of the pieces, so
+  // their places in shared memory and in the cache are a constant apart.
+  constexpr int CPR = HD / 8, RS = 128 / CPR;  // 16-byte pieces per row, rows per pass of the CTA
+  static_assert(RS % 8 == 0, "the permutation repeats every eight rows");
+  const int r0 = tid / CPR, c8 = tid % CPR, at0 = ap_at<HD>(r0, c8);
   auto issue = [&](int b) {
-    const __half* kb = b < nb1 ? keys.k : keys.k2;
-    const __half* vb = b < nb1 ? keys.v : keys.v2;
-    const int k0 = first(b), k1 = end(b);
-    __half* kd = buf + (b & 1) * 2 * TILE;
-    __half* vd = kd + TILE;
-    constexpr int CPR = HD / 8;  // 16-byte pieces per row
+    __half* kd = buf + (b & 1) * 2 * TILE + at0;
+    const int k0 = first(b), left = end(b) - k0 - r0;  // rows from r0 on
+    const size_t off = left > 0 ? (size_t)(k0 + r0) * HD + c8 * 8 : 0;
+    const __half* kb = (b < nb1 ? keys.k : keys.k2) + off;
+    const __half* vb = (b < nb1 ? keys.v : keys.v2) + off;
 #pragma unroll
-    for (int j = 0; j < kApKeys * CPR / 128; ++j) {
-      const int i = tid + 128 * j, r = i / CPR, c8 = i % CPR, key = k0 + r;
-      const bool ok = key < k1;
-      const size_t off = ok ? (size_t)key * HD + c8 * 8 : 0;
-      ap_cp16(kd + ap_at<HD>(r, c8), kb + off, ok);
-      ap_cp16(vd + ap_at<HD>(r, c8), vb + off, ok);
+    for (int j = 0; j < kApKeys / RS; ++j) {
+      const bool ok = j * RS < left;
+      const int step = ok ? j * RS * HD : 0;  // rows past the end are filled with zeros, not read
+      ap_cp16(kd + j * RS * HD, kb + step, ok);
+      ap_cp16(kd + TILE + j * RS * HD, vb + step, ok);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -199,12 +202,14 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
     }
     l0 = l0 * al0 + rs0;
     l1 = l1 * al1 + rs1;
+    if (__any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {  // a maximum moved (a NaN factor counts)
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) {
-      o[d][0] *= al0;
-      o[d][1] *= al0;
-      o[d][2] *= al1;
-      o[d][3] *= al1;
+      for (int d = 0; d < HD / 8; ++d) {
+        o[d][0] *= al0;
+        o[d][1] *= al0;
+        o[d][2] *= al1;
+        o[d][3] *= al1;
+      }
     }
 #pragma unroll
     for (int j = 0; j < KT / 2; ++j) {
