@@ -304,21 +304,11 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
   }
 }
 
-template <int HD>
-__device__ __forceinline__ void ap_tile_wr(int wr, const ApArgs& a, int m0, int i0, int n, int kv, const ApKeys& keys,
-                                           int split) {
-  if (wr == 1)
-    ap_tile<HD, 1>(a, m0, i0, n, kv, keys, split);
-  else if (wr == 2)
-    ap_tile<HD, 2>(a, m0, i0, n, kv, keys, split);
-  else
-    ap_tile<HD, 4>(a, m0, i0, n, kv, keys, split);
-}
-
-template <int HD>
+// WRP, WRO: warps along the rows of a prefix tile and of an own tile (WRP 0: no prefix here).
+template <int HD, int WRP, int WRO>
 __device__ __forceinline__ void ap_work(const ApArgs& a) {
   int b = blockIdx.x;
-  if (b < a.blocks_p) {  // a range of a prefix for a tile of the unit's query rows
+  if (WRP > 0 && b < a.blocks_p) {  // a range of a prefix for a tile of the unit's query rows
     // row tiles fastest: the tiles that read the same keys run together
     const int tile = b % a.tiles_p;
     b /= a.tiles_p;
@@ -334,7 +324,7 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
     if (j0 >= j1) return;
     const size_t base = ((size_t)u.z * a.nkv + kv) * a.prefix_cap * HD;
-    ap_tile_wr<HD>(a.wr_p, a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
+    ap_tile<HD, WRP ? WRP : 1>(a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
                    split);
     return;
   }
@@ -349,7 +339,8 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     if (threadIdx.x == 0) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
     return;
   }
-  const int tr = 16 * a.wr_o, i0 = tile * tr, n = min(tr, a.G - i0);
+  constexpr int tr = 16 * WRO;
+  const int i0 = tile * tr, n = min(tr, a.G - i0);
   const int per = ap_range(len, a.S_o), j0 = split * per, j1 = min(len, j0 + per);
   if (j0 >= j1) {
     if (a.direct && len == 0)  // nothing to attend to
@@ -359,18 +350,18 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
   float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
+  ap_tile<HD, WRO>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
                  a.S_p + split);
 }
 
-template <int HD>
+template <int HD, int WRP, int WRO>
 __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
   pdl_trigger();
   // Beside the prefix's own kernel, launched just before: that kernel waited for everything
   // earlier before it let this one start, and the two share no output, so they run together.
   // One CTA stays until it has ended, so that whoever waits for this grid waits for both.
   if (!a.tc) pdl_wait();
-  ap_work<HD>(a);
+  ap_work<HD, WRP, WRO>(a);
   if (a.tc && blockIdx.x == 0) pdl_wait();
 }
 
@@ -413,7 +404,7 @@ __device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int
 
 // Few rows and few keys: a CTA takes one row's G heads of a K/V head through the prefix and the
 // own entries and writes the output itself, in one launch.
-template <int HD>
+template <int HD, int WRO>
 __global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a) {
   pdl_trigger();
   pdl_wait();
@@ -427,7 +418,8 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a)
   const bool row = ap_row(a, m, slot, len);
   if (!row && threadIdx.x == 0) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
   if (!ap_row_prefix(a, m, pslot, plen) || !row) return;
-  const int tr = 16 * a.wr_o, i0 = tile * tr, n = min(tr, a.G - i0);
+  constexpr int tr = 16 * WRO;
+  const int i0 = tile * tr, n = min(tr, a.G - i0);
   if (plen + len == 0) {  // nothing to attend to
     for (int i = threadIdx.x; i < n * HD; i += 128)
       a.out[((size_t)m * a.nh + kv * a.G + i0) * HD + i] = __float2half_rn(0.f);
@@ -435,7 +427,7 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a)
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD, pb = ((size_t)pslot * a.nkv + kv) * a.prefix_cap * HD;
   float* srow = a.mass && len > 0 ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile_wr<HD>(a.wr_o, a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
+  ap_tile<HD, WRO>(a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
 }
 
 template <int V>
@@ -614,7 +606,7 @@ struct ApPlan {
 };
 
 constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V heads, keys of a row: one launch
-constexpr int kApTcFrom = 32;  // query rows of a unit above which its prefix takes the tcgen05 tiles
+constexpr int kApTcFrom = 32;  // query rows of a unit (one or two warps' tiles) above which its prefix takes the tcgen05 tiles
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
@@ -675,32 +667,32 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   return p;
 }
 
-template <int HD>
-int ap_launch(ApArgs a, cudaStream_t st) {
+template <int HD, int WRP, int WRO>
+int ap_launch_wr(ApArgs a, cudaStream_t st) {
   constexpr int kSmem = 4 * kApKeys * HD * 2;
   constexpr int kJoin = 64 * (HD + 4) * 4 + 64 * 8;  // WK x TR = 64 rows of O and their statistics
   constexpr int smem = kSmem > kJoin ? kSmem : kJoin;
   static bool attr_done[64] = {};
   const int dev = device_index();
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD, WRP, WRO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD, WRO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_done[dev] = true;
   }
   const dim3 none(0, 0, 0);
+  if (a.row) {
+    ORCH_CUDA(launch_k_serial(attn_prefix_row_kernel<HD, WRO>, dim3((unsigned)(a.M * a.nkv * a.tiles_o)), dim3(128), smem,
+                              st, none, a));
+    return check_launch("attention_prefix");
+  }
   if (a.tc) {
     const int rc = ap_tc_launch(a, HD, st);
     if (rc != ORCH_OK) return rc;
     a.blocks_p = 0;
   }
-  if (a.row) {
-    ORCH_CUDA(launch_k_serial(attn_prefix_row_kernel<HD>, dim3((unsigned)(a.M * a.nkv * a.tiles_o)), dim3(128), smem, st,
-                              none, a));
-    return check_launch("attention_prefix");
-  }
   const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
-  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
+  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
   if (a.direct) return check_launch("attention_prefix");
   const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
   const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
@@ -709,6 +701,21 @@ int ap_launch(ApArgs a, cudaStream_t st) {
   ORCH_CUDA(launch_k(attn_prefix_join_kernel<HD>, dim3((unsigned)jb), dim3(128), 0, st, none, a, blocks_out,
                      std::max(chunks, 1)));
   return check_launch("attention_prefix");
+}
+
+// A tile of a unit has at least the rows of a tile of one row, so wr_p >= wr_o; with head_dim 64
+// or 128 a prefix tile of 64 rows runs on tcgen05 instead.
+template <int HD>
+int ap_launch(const ApArgs& a, cudaStream_t st) {
+  const int p = a.tc || a.row || a.blocks_p == 0 ? 0 : a.wr_p;
+  if (p == 0)
+    return a.wr_o == 1 ? ap_launch_wr<HD, 0, 1>(a, st) : a.wr_o == 2 ? ap_launch_wr<HD, 0, 2>(a, st) : ap_launch_wr<HD, 0, 4>(a, st);
+  if (p == 1) return ap_launch_wr<HD, 1, 1>(a, st);
+  if (p == 2) return a.wr_o == 1 ? ap_launch_wr<HD, 2, 1>(a, st) : ap_launch_wr<HD, 2, 2>(a, st);
+  if constexpr (HD == 32)
+    return a.wr_o == 1 ? ap_launch_wr<HD, 4, 1>(a, st) : a.wr_o == 2 ? ap_launch_wr<HD, 4, 2>(a, st) : ap_launch_wr<HD, 4, 4>(a, st);
+  else
+    return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: no kernel for this tile");
 }
 
 bool ap_shape_ok(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd) {
