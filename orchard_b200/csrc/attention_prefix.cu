@@ -13,9 +13,11 @@
 // that K/V head), so the prefix is read once for all of them; another CTA takes a range of
 // one row's own entries for its G heads. Both run the same tensor-core tile: S = Q K^T in
 // m16n8k16 MMAs (exact products of fp16 values, fp32 sums), an online softmax in fp32, O += P V
-// with P rounded to fp16. That rounding costs 2^-12 relative per weight, below the rounding of
-// the fp16 output; P is scaled by 2^10 so that weights down to 2^-24 of the largest stay
-// normal numbers. The sums l take the unrounded weights.
+// with P rounded to fp16. That rounding costs up to 2^-11 of each weight, as much as the rounding
+// of the fp16 output; the sums l take the unrounded weights, and P is scaled by 2^10 so that
+// weights down to 2^-24 of the largest stay normal numbers. With few rows (`fine`), where the
+// products are not what takes the time, P V adds what the rounding left off as a second product
+// (64 rows behind 4,096 entries: 65.6 us without, 70.4 with; one row of 577: 9.0 and 9.2).
 //
 // Layout of a CTA: 4 warps. A tile of 64 rows gives each warp 16 rows and all 64 keys of a
 // block; a tile of 16 or 32 rows splits the block's keys over 4 or 2 warps instead, whose
@@ -67,7 +69,7 @@ struct ApKeys {
 
 // One tile: query rows i0 .. i0 + n - 1 of the (row, head of kv) pairs starting at row m0, over
 // `keys`; partials go to range `split`. The statistics of the rows stay in shared memory.
-template <int HD, int WR>
+template <int HD, int WR, bool FINE>
 __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, int kv, const ApKeys& keys, int split) {
   constexpr int WK = 4 / WR, TR = 16 * WR, TILE = kApKeys * HD, KT = kApKeys / 8 / WK;
   extern __shared__ __align__(16) uint8_t ap_smem[];
@@ -213,17 +215,27 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
     }
 #pragma unroll
     for (int j = 0; j < KT / 2; ++j) {
-      uint32_t pa[4];
-      pa[0] = h2_bits(__floats2half2_rn(sc[2 * j][0], sc[2 * j][1]));
-      pa[1] = h2_bits(__floats2half2_rn(sc[2 * j][2], sc[2 * j][3]));
-      pa[2] = h2_bits(__floats2half2_rn(sc[2 * j + 1][0], sc[2 * j + 1][1]));
-      pa[3] = h2_bits(__floats2half2_rn(sc[2 * j + 1][2], sc[2 * j + 1][3]));
+      uint32_t hi[4], lo[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float p0 = sc[2 * j + (x >> 1)][2 * (x & 1)], p1 = sc[2 * j + (x >> 1)][2 * (x & 1) + 1];
+        const __half2 h = __floats2half2_rn(p0, p1);
+        hi[x] = h2_bits(h);
+        if (FINE) {
+          const float2 f = __half22float2(h);
+          lo[x] = h2_bits(__floats2half2_rn(p0 - f.x, p1 - f.y));
+        }
+      }
 #pragma unroll
       for (int d = 0; d < HD / 8; d += 2) {
         uint32_t bb[4];
         ap_ldsm4_t(vs + ap_at<HD>(8 * kt0 + 16 * j + 8 * (lm & 1) + lr, d + (lm >> 1)), bb);
-        mma_16816(o[d], pa[0], pa[1], pa[2], pa[3], bb[0], bb[1]);
-        mma_16816(o[d + 1], pa[0], pa[1], pa[2], pa[3], bb[2], bb[3]);
+        mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], bb[0], bb[1]);
+        mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], bb[2], bb[3]);
+        if (FINE) {
+          mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
+          mma_16816(o[d + 1], lo[0], lo[1], lo[2], lo[3], bb[2], bb[3]);
+        }
       }
     }
     __syncthreads();  // buffer b & 1 is free for block b + 2
@@ -305,7 +317,8 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 }
 
 // WRP, WRO: warps along the rows of a prefix tile and of an own tile (WRP 0: no prefix here).
-template <int HD, int WRP, int WRO>
+// FINE: weights in two fp16 terms.
+template <int HD, int WRP, int WRO, bool FINE>
 __device__ __forceinline__ void ap_work(const ApArgs& a) {
   int b = blockIdx.x;
   if (WRP > 0 && b < a.blocks_p) {  // a range of a prefix for a tile of the unit's query rows
@@ -324,7 +337,7 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
     if (j0 >= j1) return;
     const size_t base = ((size_t)u.z * a.nkv + kv) * a.prefix_cap * HD;
-    ap_tile<HD, WRP ? WRP : 1>(a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
+    ap_tile<HD, WRP ? WRP : 1, FINE>(a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
                    split);
     return;
   }
@@ -350,18 +363,18 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
   float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile<HD, WRO>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
+  ap_tile<HD, WRO, FINE>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
                  a.S_p + split);
 }
 
-template <int HD, int WRP, int WRO>
+template <int HD, int WRP, int WRO, bool FINE>
 __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
   pdl_trigger();
   // Beside the prefix's own kernel, launched just before: that kernel waited for everything
   // earlier before it let this one start, and the two share no output, so they run together.
   // One CTA stays until it has ended, so that whoever waits for this grid waits for both.
   if (!a.tc) pdl_wait();
-  ap_work<HD, WRP, WRO>(a);
+  ap_work<HD, WRP, WRO, FINE>(a);
   if (a.tc && blockIdx.x == 0) pdl_wait();
 }
 
@@ -427,7 +440,7 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a)
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD, pb = ((size_t)pslot * a.nkv + kv) * a.prefix_cap * HD;
   float* srow = a.mass && len > 0 ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile<HD, WRO>(a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
+  ap_tile<HD, WRO, true>(a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
 }
 
 template <int V>
@@ -667,15 +680,15 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   return p;
 }
 
-template <int HD, int WRP, int WRO>
-int ap_launch_wr(ApArgs a, cudaStream_t st) {
+template <int HD, int WRP, int WRO, bool FINE>
+int ap_launch_shape(ApArgs a, cudaStream_t st) {
   constexpr int kSmem = 4 * kApKeys * HD * 2;
   constexpr int kJoin = 64 * (HD + 4) * 4 + 64 * 8;  // WK x TR = 64 rows of O and their statistics
   constexpr int smem = kSmem > kJoin ? kSmem : kJoin;
   static bool attr_done[64] = {};
   const int dev = device_index();
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD, WRP, WRO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD, WRP, WRO, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD, WRO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_done[dev] = true;
   }
@@ -692,7 +705,7 @@ int ap_launch_wr(ApArgs a, cudaStream_t st) {
   }
   const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
-  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
+  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO, FINE>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
   if (a.direct) return check_launch("attention_prefix");
   const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
   const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
@@ -701,6 +714,11 @@ int ap_launch_wr(ApArgs a, cudaStream_t st) {
   ORCH_CUDA(launch_k(attn_prefix_join_kernel<HD>, dim3((unsigned)jb), dim3(128), 0, st, none, a, blocks_out,
                      std::max(chunks, 1)));
   return check_launch("attention_prefix");
+}
+
+template <int HD, int WRP, int WRO>
+int ap_launch_wr(const ApArgs& a, cudaStream_t st) {
+  return a.fine ? ap_launch_shape<HD, WRP, WRO, true>(a, st) : ap_launch_shape<HD, WRP, WRO, false>(a, st);
 }
 
 // A tile of a unit has at least the rows of a tile of one row, so wr_p >= wr_o; with head_dim 64
@@ -802,6 +820,7 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.blocks_p = (int)blocks_p;
   a.direct = p.direct;
   a.row = p.row;
+  a.fine = (uint64_t)M * num_kv_heads <= kApDirectPairs;
   a.acc = static_cast<float*>(workspace);
   a.stat = reinterpret_cast<float2*>(a.acc + p.acc_floats);
   a.scores = a.acc + p.acc_floats + p.stat_floats;
