@@ -448,25 +448,28 @@ struct alignas(4 * V) ApVec {
   float v[V];
 };
 
-// The common maximum and sum of row-head mh over its ranges. (Called by whole warps.)
-__device__ __forceinline__ float2 ap_total(const ApArgs& a, size_t mh, int np, int no) {
-  const int lane = threadIdx.x & 31;
-  const float2* st = a.stat + mh * (a.S_p + a.S_o);
-  float mx = -INFINITY;
-  for (int s = lane; s < np + no; s += 32) mx = fmaxf(mx, st[s < np ? s : a.S_p + s - np].x);
+// The common maximum and sum of row-head mh over its ranges; `first` is this lane's record (range
+// `lane`), read before it was known which ranges hold keys. (Called by whole warps.)
+__device__ __forceinline__ float2 ap_total(const ApArgs& a, size_t mh, int np, int no, float2 first) {
+  const int lane = threadIdx.x & 31, S = a.S_p + a.S_o;
+  const float2* st = a.stat + mh * S;
+  auto live = [&](int s) { return s < np || (s >= a.S_p && s < a.S_p + no); };
+  if (lane >= S || !live(lane)) first = make_float2(-INFINITY, 0.f);
+  float mx = first.x;
+  for (int s = lane + 32; s < S; s += 32)
+    if (live(s)) mx = fmaxf(mx, st[s].x);
   mx = warp_max(mx);
-  float l = 0.f;
-  for (int s = lane; s < np + no; s += 32) {
-    const float2 v = st[s < np ? s : a.S_p + s - np];
-    l += v.x == -INFINITY ? v.y : ap_exp2(v.x - mx) * v.y;
-  }
+  // a range whose maximum is -inf has sum 0, or NaN where a key was NaN: that one is kept
+  float l = first.x == -INFINITY ? first.y : ap_exp2(first.x - mx) * first.y;
+  for (int s = lane + 32; s < S; s += 32)
+    if (live(s)) l += st[s].x == -INFINITY ? st[s].y : ap_exp2(st[s].x - mx) * st[s].y;
   return make_float2(mx, warp_sum(l));
 }
 
 // Joins the ranges: one warp per (row, head) for the output; with mass, further CTAs each
 // take kMassEntries entries of one (row, K/V head).
 constexpr int kMassEntries = 512;
-constexpr int kMassHeads = 4;  // heads of a K/V head taken at once
+constexpr int kMassHeads = 4;  // heads of a K/V head taken at once, a warp each
 
 template <int HD>
 __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, int blocks_out, int chunks) {
@@ -490,18 +493,9 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
     int slot, len, np, no;
     if (!ap_ranges(a, mh / a.nh, slot, len, np, no)) return;
     auto live = [&](int s) { return s < np || (s >= a.S_p && s < a.S_p + no); };
-    if (!live(lane)) sl = make_float2(-INFINITY, 0.f);
-    float mx = sl.x;
-    for (int s = lane + 32; s < S; s += 32)
-      if (live(s)) mx = fmaxf(mx, st[s].x);
-    mx = warp_max(mx);
-    auto weight = [&](float m) { return m == -INFINITY ? 0.f : ap_exp2(m - mx); };
-    const float wl = weight(sl.x);
-    // a range whose maximum is -inf has sum 0, or NaN where a key was NaN: that one is kept
-    float l = sl.x == -INFINITY ? sl.y : wl * sl.y;
-    for (int s = lane + 32; s < S; s += 32)
-      if (live(s)) l += st[s].x == -INFINITY ? st[s].y : weight(st[s].x) * st[s].y;
-    l = warp_sum(l);
+    const float2 tot = ap_total(a, mh, np, no, sl);
+    auto weight = [&](float m) { return m == -INFINITY ? 0.f : ap_exp2(m - tot.x); };
+    const float wl = lane < S && live(lane) ? weight(sl.x) : 0.f;
     float v[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = 0.f;
@@ -521,7 +515,6 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
         for (int i = 0; i < V; ++i) v[i] = fmaf(f, x.v[i], v[i]);
       }
     }
-    const float2 tot = make_float2(mx, l);
     const float inv = tot.y == 0.f ? 0.f : 1.0f / tot.y;  // nothing to attend to: zeros
     __half* op = a.out + (size_t)mh * HD + lane * V;
     if (V == 4) {
@@ -558,10 +551,22 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
         sv[j][i] = j < a.G - h0 && e < len ? sr[(size_t)j * a.lds + e] : -INFINITY;
       }
   };
-  fetch(m, 0);
   __shared__ int any;
   __shared__ float2 tots[kMassHeads];
   if (threadIdx.x == 0) any = 0;
+  // requested before anything is known of other rows: this row's scores and records, the masses
+  fetch(m, 0);
+  const int S1 = a.S_p + a.S_o;
+  auto record = [&](int r, int h) {
+    return h < a.G && lane < S1 ? a.stat[((size_t)r * a.nh + kv * a.G + h) * S1 + lane] : make_float2(0.f, 0.f);
+  };
+  float2 rec = record(m, warp);
+  float old[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int e = e0 + threadIdx.x + 128 * i;
+    old[i] = e < len ? mass[e] : 0.f;
+  }
   __syncthreads();
   int mine = 0;  // whether another row of the call has this slot: 1 an earlier one, 2 a later one
   for (int r = threadIdx.x; r < a.M; r += 128)
@@ -582,6 +587,12 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
       int s2;
       if ((a.slots ? a.slots[r] : r) != slot || !ap_ranges(a, r, s2, len, np, no) || e0 >= len) continue;
       fetch(r, 0);
+      rec = record(r, warp);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {  // what the rows before have left there
+        const int e = e0 + threadIdx.x + 128 * i;
+        old[i] = e < len ? mass[e] : 0.f;
+      }
     } else if (e0 >= len) {
       continue;
     }
@@ -592,9 +603,10 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
       const int hs = min(kMassHeads, a.G - h0);
       if (h0 > 0) fetch(r, h0);
       __syncthreads();  // the totals of the heads before are done with
-      for (int j = warp; j < hs; j += 4) {  // the heads' totals, a warp each
-        const float2 tot = ap_total(a, (size_t)r * a.nh + kv * a.G + h0 + j, np, no);
-        if (lane == 0) tots[j] = make_float2(tot.x == -INFINITY ? 0.f : tot.x - kApShift, tot.y == 0.f ? 0.f : 1.0f / tot.y);
+      if (h0 > 0) rec = record(r, h0 + warp);
+      if (warp < hs) {  // the heads' totals, a warp each
+        const float2 tot = ap_total(a, (size_t)r * a.nh + kv * a.G + h0 + warp, np, no, rec);
+        if (lane == 0) tots[warp] = make_float2(tot.x == -INFINITY ? 0.f : tot.x - kApShift, tot.y == 0.f ? 0.f : 1.0f / tot.y);
       }
       __syncthreads();
 #pragma unroll
@@ -606,7 +618,7 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int e = e0 + threadIdx.x + 128 * i;
-      if (e < len) mass[e] = e == len - 1 ? w[i] : mass[e] + w[i];
+      if (e < len) mass[e] = e == len - 1 ? w[i] : old[i] + w[i];
     }
   }
 }
