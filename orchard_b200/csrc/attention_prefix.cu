@@ -651,7 +651,10 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.tiles_p = some ? (int)((q_rows + (size_t)num_units * (p.tr_p - 1)) / p.tr_p) : 0;
   const size_t likely = std::max<size_t>((q_rows + p.tr_p - 1) / p.tr_p, num_units);
   p.tiles_o = (p.G + 16 * p.wr_o - 1) / (16 * p.wr_o);
-  const int want = 6 * num_sms();  // two rounds of three CTAs per SM
+  // Two rounds of three CTAs per SM at most; ranges long enough to pay for their start and their
+  // record, shorter ones only where there are few CTAs (16 x 32 heads, prefix 1,000, own entries up
+  // to 128: 12.8 us with ranges of 256 and 128 keys at least, 15.7 with 128 and 64).
+  const int want = 6 * num_sms();
   const auto ranges = [&](size_t ctas, uint32_t keys, int least) {
     const size_t s = (want + ctas - 1) / std::max<size_t>(ctas, 1);
     return (int)std::max<size_t>(1, std::min<size_t>(s, (keys + least - 1) / least));
@@ -673,9 +676,10 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
       if (p.S_p == 0 || cost < best) p.S_p = c, best = cost;
     }
   } else if (some) {
-    p.S_p = ranges(items, max_prefix, 64 * p.wr_p + 64);
+    p.S_p = ranges(items, max_prefix, items * (max_prefix / 256) >= (size_t)num_sms() / 2 ? 256 : 128);
   }
-  p.S_o = ranges((size_t)M * nkv * p.tiles_o, max_own, 64);  // at least one: rows are checked there
+  const size_t own_items = (size_t)M * nkv * p.tiles_o;
+  p.S_o = ranges(own_items, max_own, own_items >= (size_t)num_sms() ? 128 : 64);
   // Few CTAs with little to read: splitting would cost a second launch and more than it saves (2 x
   // 2 heads of 32 keys: 3.2 us in one launch, 4.9 in two; one row of 32 heads x 577 keys, tracked:
   // 15.9 and 9.7). Weights only for a single row: rows that share a slot need an order.
