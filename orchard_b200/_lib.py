@@ -153,6 +153,19 @@ def last_error() -> str:
 
 
 _fns = {}  # name -> typed entry point, filled at its first call
+_entries = {}  # name -> CPython entry point (csrc/entry.cpp), where there is one
+
+
+def _load_entries():
+    """The CPython entry points, once the library itself is loaded; ctypes serves every name where
+    they were not built."""
+    lib()
+    try:
+        from . import _entry
+    except ImportError:
+        _entries[""] = None
+        return
+    _entries.update({n: getattr(_entry, n) for n in dir(_entry) if n.startswith("orch_")})
 
 
 def call(name: str, *args) -> int:
@@ -161,6 +174,14 @@ def call(name: str, *args) -> int:
     Tensor arguments are passed by device address and stay referenced for the duration of
     the call; work enqueued on a stream is ordered before any later reuse of their memory
     by the caching allocator on that stream."""
+    if not _entries:
+        _load_entries()
+    f = _entries.get(name)
+    if f is not None:
+        rc = f(*args)
+        if rc != 0:
+            raise OrchardError(name, rc, last_error())
+        return rc
     f = _fns.get(name)
     if f is None:
         f = _fns[name] = getattr(lib(), name)

@@ -5,6 +5,7 @@
 * ``orchard_b200/orchard_core<ext>`` -- the pybind11 module with the reference's
   operator surface (``MetalBackend``, ``Tensor``, ``DType``; src/bindings.cpp), linked
   against the library above with an ``$ORIGIN`` rpath.
+* ``orchard_b200/_entry<ext>`` -- CPython entry points of the serving operators.
 
 Usage: ``python -m orchard_b200.build [--force] [-j N]``.
 """
@@ -100,9 +101,27 @@ def build_core(force=False):
     return target
 
 
+def entry_ext_path():
+    suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+    return os.path.join(PKG, "_entry" + suffix)
+
+
+def build_entry(force=False):
+    """CPython entry points of the serving operators, linked to the C ABI."""
+    target = entry_ext_path()
+    src = os.path.join(CSRC, "entry.cpp")
+    if not force and not _stale(target, [src] + _headers() + [LIB]):
+        return target
+    _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+          "-I", sysconfig.get_paths()["include"], "-I", os.path.join(ROOT, "include"), src, "-o", target,
+          "-L", LIBDIR, "-lorchard_b200", "-Wl,-rpath,$ORIGIN/lib"])
+    return target
+
+
 def build_all(force=False, jobs=8, verbose=False):
     build_lib(force=force, jobs=jobs, verbose=verbose)
     build_core(force=force)
+    build_entry(force=force)
     return LIB
 
 

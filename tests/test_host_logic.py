@@ -98,3 +98,35 @@ def test_prefix_units_cover_the_rows():
         assert u[:, 1].max() <= 128 and u[:, 1].min() >= 1
         np.testing.assert_array_equal(np.concatenate([np.arange(a, a + n) for a, n, _, _ in u]), np.arange(rows))
     assert serving.prefix_units(0, 0, 1).shape == (0, 4)
+
+
+def test_entry_points_convert_and_report_like_ctypes():
+    """The CPython entry points of the serving operators: built, declared in the header, the same
+    statuses and messages as through ctypes, and no call with a wrong argument."""
+    import pytest
+    from orchard_b200 import _lib
+    _lib._load_entries()
+    names = [n for n in _lib._entries if n]
+    assert set(names) == {"orch_attention_prefix", "orch_cache_evict", "orch_logits_process", "orch_q4t_qkv_rope_at",
+                          "orch_q4t_rms_qkv_rope_at"} <= set(_lib.header_symbols())
+    for n in names:
+        assert len(_lib._SIGS[n][1]) > 10
+        with pytest.raises(TypeError, match="arguments"):
+            _lib._entries[n](1, 2, 3)
+        count = len(_lib._SIGS[n][1])
+        m = [i for i, a in enumerate(_lib._SIGS[n][1]) if a is _lib._u32]
+        args = [None if a is _lib._vp else 0 for a in _lib._SIGS[n][1]]
+        assert len(args) == count and _lib.call(n, *args) == 0  # no rows: nothing to do
+        args = [1 if i in m else a for i, a in enumerate(args)]
+        with pytest.raises(_lib.OrchardError, match="null") as e:
+            _lib.call(n, *args)
+        assert e.value.status == getattr(_lib.lib(), n)(*args) == 1
+        args[0] = object()
+        with pytest.raises(AttributeError):
+            _lib.call(n, *args)
+        args[0], args[m[0]] = None, "1"
+        with pytest.raises(TypeError):
+            _lib.call(n, *args)
+    x = torch.zeros(4)
+    with pytest.raises(_lib.OrchardError, match="null"):  # a tensor by its address, numpy whole numbers
+        _lib.call("orch_cache_evict", x, x, x, x, x, None, x, x, None, np.int64(1), 1, 8, 8, 1, 4, 1, None)
