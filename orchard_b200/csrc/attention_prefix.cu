@@ -648,7 +648,7 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.tr_p = !p.tc ? 16 * p.wr_p : rows_p > kApTcRows ? 2 * kApTcRows : kApTcRows;
   // the units share out at most M rows: their tiles are at most this many, and about `likely`
   const size_t q_rows = (size_t)M * p.G;
-  p.tiles_p = some ? (int)((q_rows + (size_t)num_units * (p.tr_p - 1)) / p.tr_p) : 0;
+  p.tiles_p = some ? (int)std::min<size_t>((q_rows + (size_t)num_units * (p.tr_p - 1)) / p.tr_p, 0x7fffffff) : 0;
   const size_t likely = std::max<size_t>((q_rows + p.tr_p - 1) / p.tr_p, num_units);
   p.tiles_o = (p.G + 16 * p.wr_o - 1) / (16 * p.wr_o);
   // Two rounds of three CTAs per SM at most; ranges long enough to pay for their start and their
@@ -787,9 +787,9 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   ORCH_REQUIRE(max_seq > 0 && max_seq <= kApMaxLen && num_slots > 0 && num_slots <= 0x7fffffffu && max_own <= max_seq,
                "attention_prefix: bad cache shape (max_own must not exceed max_seq)");
   ORCH_REQUIRE(num_units == 0 || max_prefix == 0 ||
-                   (max_prefix <= prefix_cap && prefix_cap <= kApMaxLen && num_prefix > 0 && num_prefix <= 0x7fffffffu &&
-                    num_units <= 0x7fffffffu),
+                   (max_prefix <= prefix_cap && prefix_cap <= kApMaxLen && num_prefix > 0 && num_prefix <= 0x7fffffffu),
                "attention_prefix: bad prefix shape (max_prefix must not exceed prefix_cap)");
+  ORCH_REQUIRE(num_units <= M, "attention_prefix: more units than rows (a row belongs to one at most)");
   ORCH_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)prefix_k |
                  (uintptr_t)prefix_v | (uintptr_t)units | (uintptr_t)workspace) & 15) == 0,
                "attention_prefix: buffers must be 16-byte aligned");

@@ -232,6 +232,49 @@ def test_prefix_attention_repeats_and_serves_a_captured_graph():
     check_attention((q, kp, vp, units, kc, vc, lens, slots), got=out)
 
 
+@pytest.mark.parametrize("rows,nh,nkv", [(64, 4, 4), (70, 8, 2)])
+def test_captured_calls_in_a_row(rows, nh, nkv):
+    """Units of more than 32 query rows (the prefix in a kernel of its own beside the own entries'):
+    several calls that share a workspace, captured back to back and replayed with other lengths,
+    weights added up in call order."""
+    lens = [(11 * i) % 60 for i in range(rows)]
+    q, kp, vp, units, kc, vc, lens, slots = case(70, 128, nh, nkv, [(0, rows, 0, 900)], lens, 64, pcap=900, poison=False)
+    t = [D(x) for x in (q, kp, vp, units, kc, vc, lens, slots)]
+    mass = torch.zeros((rows, nkv, 64), device="cuda")
+    outs = [torch.zeros((rows, nh, 128), dtype=torch.float16, device="cuda") for _ in range(4)]
+    n = _lib.lib().orch_attention_prefix_workspace_bytes(rows, nh, nkv, 128, 1, 900, 64, 1)
+    ws = torch.zeros(n // 4 + 4, device="cuda")
+    q2 = t[0].flip(0).contiguous()
+
+    def calls():
+        for i, o in enumerate(outs):
+            call("orch_attention_prefix", q2 if i % 2 else t[0], t[1], t[2], t[3], 1, 900, 900, 1, t[4], t[5], t[6], t[7], 64,
+                 64, rows, mass, o, rows, nh, nkv, 128, ws, n, S())
+
+    calls()
+    torch.cuda.synchronize()
+    mass.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        calls()
+    for step in range(2):
+        if step:
+            units[0, 3], lens = 513, np.asarray([(7 * i + 3) % 65 for i in range(rows)], np.int32)
+            t[3].copy_(D(units))
+            t[6].copy_(D(lens))
+        mass.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        check_attention((q, kp, vp, units, kc, vc, lens, slots), got=outs[0])
+        check_attention((q[::-1].copy(), kp, vp, units, kc, vc, lens, slots), got=outs[1])
+        assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
+        want = np.zeros((rows, nkv, 64), np.float64)
+        for qq in (q, q[::-1], q, q[::-1]):
+            _, _, want, big = serving.attention_prefix(qq, kp, vp, units, kc, vc, lens, slots, want)
+        rel = 2 * 2.0 ** -19 * big + 2.0 ** -19
+        assert np.all(np.abs(mass.double().cpu().numpy() - want) <= rel * np.abs(want) + 1e-30)
+
+
 @pytest.mark.parametrize("track,cap", [(True, 10), (False, 10), (False, 700)])
 def test_prefix_attention_skips_bad_rows_and_units(track, cap):
     q, kp, vp, units, kc, vc, lens, slots = case(50, 64, 4, 2, [(0, 2, 0, 30), (2, 2, 0, 30), (4, 2, 0, 30)], [3, 4, 5, 6, 7, 8],

@@ -38,7 +38,7 @@ def logits(**kw):
     (dict(kp=None), b"null prefix"), (dict(units=None), b"null prefix"), (dict(nkv=3), b"multiple"), (dict(nkv=0), b"multiple"),
     (dict(hd=48), b"head_dim"), (dict(hd=256), b"head_dim"), (dict(mo=9), b"max_own"), (dict(ns=0), b"cache shape"),
     (dict(cap=0, mo=0), b"cache shape"), (dict(cap=2 ** 30), b"cache shape"), (dict(mp=9), b"max_prefix"),
-    (dict(np_=0), b"prefix shape"), (dict(q=P + 2), b"aligned"), (dict(units=P + 4), b"aligned"), (dict(ws=P + 8, wb=1 << 30), b"aligned"),
+    (dict(np_=0), b"prefix shape"), (dict(nu=2), b"units"), (dict(q=P + 2), b"aligned"), (dict(units=P + 4), b"aligned"), (dict(ws=P + 8, wb=1 << 30), b"aligned"),
     (dict(ws=None, mo=4000, cap=4000), b"workspace"), (dict(ws=P, wb=16, mo=4000, cap=4000), b"workspace")])
 def test_attention_refusals(kw, word):
     assert attention(**kw) == 1 and word in _lib.lib().orch_last_error()
