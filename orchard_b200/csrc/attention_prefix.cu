@@ -631,7 +631,11 @@ struct ApPlan {
 };
 
 constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V heads, keys of a row: one launch
-constexpr int kApTcFrom = 32;  // query rows of a unit (one or two warps' tiles) above which its prefix takes the tcgen05 tiles
+// Query rows of a unit, and blocks of 128 x 128 (rows, keys) over all heads, from which the prefix
+// takes the tcgen05 tiles. A third launch and their start cost ~5 us: 16 rows x 8 heads x 4 behind
+// 2,048 entries (128 blocks) 16.5 us with them, 12.0 without; 64 x 32 heads behind 512 (128 blocks)
+// 25.2 and 24.7, behind 1,024 26.1 and 28.0, behind 4,096 65.8 and 80.
+constexpr int kApTcFrom = 32, kApTcBlocks = 256;
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
@@ -641,9 +645,10 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.G = (int)(nh / nkv);
   const int rows_p = (int)std::min<uint32_t>(M, kApMaxUnitRows) * p.G;
   const bool some = num_units > 0 && max_prefix > 0;
-  p.tc = some && hd != 32 && rows_p > kApTcFrom;
+  p.tc = some && hd != 32 && rows_p > kApTcFrom &&
+         nkv * (((size_t)M * p.G + 127) / 128) * ((max_prefix + 127) / 128) >= (size_t)kApTcBlocks;
   p.blk_p = p.tc ? kApTcKeys : kApKeys;
-  p.wr_p = ap_wr(rows_p);
+  p.wr_p = std::min(ap_wr(rows_p), hd == 32 || p.G > 32 ? 4 : 2);  // 64 rows of 64 or 128 dims spill
   p.wr_o = ap_wr(p.G);
   p.tr_p = !p.tc ? 16 * p.wr_p : rows_p > kApTcRows ? 2 * kApTcRows : kApTcRows;
   // the units share out at most M rows: their tiles are at most this many, and about `likely`
@@ -738,7 +743,7 @@ int ap_launch_wr(const ApArgs& a, cudaStream_t st) {
 }
 
 // A tile of a unit has at least the rows of a tile of one row, so wr_p >= wr_o; with head_dim 64
-// or 128 a prefix tile of 64 rows runs on tcgen05 instead.
+// or 128 it has 64 rows only where a row's heads already fill that.
 template <int HD>
 int ap_launch(const ApArgs& a, cudaStream_t st) {
   const int p = a.tc || a.row || a.blocks_p == 0 ? 0 : a.wr_p;
@@ -746,10 +751,11 @@ int ap_launch(const ApArgs& a, cudaStream_t st) {
     return a.wr_o == 1 ? ap_launch_wr<HD, 0, 1>(a, st) : a.wr_o == 2 ? ap_launch_wr<HD, 0, 2>(a, st) : ap_launch_wr<HD, 0, 4>(a, st);
   if (p == 1) return ap_launch_wr<HD, 1, 1>(a, st);
   if (p == 2) return a.wr_o == 1 ? ap_launch_wr<HD, 2, 1>(a, st) : ap_launch_wr<HD, 2, 2>(a, st);
-  if constexpr (HD == 32)
-    return a.wr_o == 1 ? ap_launch_wr<HD, 4, 1>(a, st) : a.wr_o == 2 ? ap_launch_wr<HD, 4, 2>(a, st) : ap_launch_wr<HD, 4, 4>(a, st);
-  else
-    return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: no kernel for this tile");
+  if constexpr (HD == 32) {
+    if (a.wr_o == 1) return ap_launch_wr<HD, 4, 1>(a, st);
+    if (a.wr_o == 2) return ap_launch_wr<HD, 4, 2>(a, st);
+  }
+  return ap_launch_wr<HD, 4, 4>(a, st);
 }
 
 bool ap_shape_ok(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd) {

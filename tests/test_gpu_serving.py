@@ -119,6 +119,19 @@ def test_prefix_rows_per_unit(rows, nh, nkv):
     check_attention(case(rows, 128, nh, nkv, [(0, rows, 0, 333)], lens, 40, pcap=340))
 
 
+@pytest.mark.parametrize("bound", [0, 40000])
+@pytest.mark.parametrize("hd,nh,nkv,rows,plen", [(128, 2, 2, 33, 1), (128, 2, 2, 64, 129), (64, 6, 2, 50, 63), (64, 20, 1, 3, 700),
+                                                 (128, 70, 1, 3, 128), (128, 4, 1, 65, 333), (64, 4, 1, 128, 1000)])
+def test_prefix_tiles_by_the_bound(hd, nh, nkv, rows, plen, bound):
+    """Both kinds of prefix tiles at the same lengths: a bound far above them asks for the tcgen05
+    tiles (blocks of 128 x 128 are counted by the bounds), whose last blocks then end anywhere."""
+    host = case(rows + plen, hd, nh, nkv, [(0, rows, 0, plen)], [(7 * i) % 40 for i in range(rows)], 40, pcap=plen + 5)
+    q, kp, vp, units, kc, vc, lens, slots = host
+    pad = np.zeros((1, nkv, max(0, bound - plen - 5), hd), np.float16)
+    t = [D(x) for x in (q, np.concatenate([kp, pad], 2), np.concatenate([vp, pad], 2), units, kc, vc, lens, slots)]
+    check_attention(host, got=attention(*t, max_prefix=max(plen, bound)))
+
+
 @pytest.mark.parametrize("rows,nh,nkv,hd,plen", [(128, 32, 32, 128, 1777), (96, 32, 8, 64, 2500), (40, 160, 160, 64, 1300)])
 def test_prefix_of_many_blocks_per_range(rows, nh, nkv, hd, plen):
     """Enough row tiles that one CTA goes through a long range; scores that grow along the keys,
@@ -232,10 +245,9 @@ def test_prefix_attention_repeats_and_serves_a_captured_graph():
     check_attention((q, kp, vp, units, kc, vc, lens, slots), got=out)
 
 
-@pytest.mark.parametrize("rows,nh,nkv", [(64, 4, 4), (70, 8, 2)])
+@pytest.mark.parametrize("rows,nh,nkv", [(64, 32, 32), (70, 44, 11), (20, 4, 4)])
 def test_captured_calls_in_a_row(rows, nh, nkv):
-    """Units of more than 32 query rows (the prefix in a kernel of its own beside the own entries'):
-    several calls that share a workspace, captured back to back and replayed with other lengths,
+    """Large units (the prefix in a kernel of its own beside the own entries') and small ones: several calls that share a workspace, captured back to back and replayed with other lengths,
     weights added up in call order."""
     lens = [(11 * i) % 60 for i in range(rows)]
     q, kp, vp, units, kc, vc, lens, slots = case(70, 128, nh, nkv, [(0, rows, 0, 900)], lens, 64, pcap=900, poison=False)
@@ -266,12 +278,18 @@ def test_captured_calls_in_a_row(rows, nh, nkv):
         g.replay()
         torch.cuda.synchronize()
         check_attention((q, kp, vp, units, kc, vc, lens, slots), got=outs[0])
-        check_attention((q[::-1].copy(), kp, vp, units, kc, vc, lens, slots), got=outs[1])
         assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3])
-        want = np.zeros((rows, nkv, 64), np.float64)
-        for qq in (q, q[::-1], q, q[::-1]):
-            _, _, want, big = serving.attention_prefix(qq, kp, vp, units, kc, vc, lens, slots, want)
-        rel = 2 * 2.0 ** -19 * big + 2.0 ** -19
+        # each call adds the same weights again, and starts the newest entry anew
+        zero = np.zeros((rows, nkv, 64), np.float64)
+        _, _, w1, big = serving.attention_prefix(q, kp, vp, units, kc, vc, lens, slots, zero)
+        o2, absv, w2, big2 = serving.attention_prefix(q[::-1], kp, vp, units, kc, vc, lens, slots, zero)
+        bound = 2.0 ** -11 * (np.abs(o2) + absv) + 2.0 ** -19 * big2 * absv + 2.0 ** -24
+        assert np.all(np.abs(outs[1].double().cpu().numpy() - o2) <= bound)
+        want = 2 * (w1 + w2)
+        for m in range(rows):
+            if lens[m]:
+                want[slots[m], :, lens[m] - 1] = w2[slots[m], :, lens[m] - 1]
+        rel = 2 * 2.0 ** -19 * max(big, big2) + 2.0 ** -19
         assert np.all(np.abs(mass.double().cpu().numpy() - want) <= rel * np.abs(want) + 1e-30)
 
 
