@@ -316,7 +316,168 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
   }
 }
 
-// WRP, WRO: warps along the rows of a prefix tile and of an own tile (WRP 0: no prefix here).
+// The same tile for one warp: the G <= 16 heads of a K/V head of row m over the row's own entries
+// [j0, j1), 16 keys at a time through the warp's own ring of two stages. Where there are enough
+// rows and heads, four of these per CTA need no barrier and no join across warps, and a quarter of
+// the CTAs: AAA.
+template <int HD, bool FINE>
+__device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __half* k, const __half* v, int j0, int j1,
+                                        int split, float* srow) {
+  constexpr int KEYS = 16, TILE = KEYS * HD, CPR = HD / 8, RS = 32 / CPR;  // 16-byte pieces per row, rows per pass
+  extern __shared__ __align__(16) uint8_t ap_smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  __half* buf = reinterpret_cast<__half*>(ap_smem) + warp * 4 * TILE;  // [stage][K, V][key][dim]
+  const int nb = (j1 - j0 + KEYS - 1) / KEYS, r0 = lane / CPR, c8 = lane % CPR, n = a.G;
+
+  auto issue = [&](int b) {
+    __half* kd = buf + (b & 1) * 2 * TILE;
+    const int left = j1 - j0 - b * KEYS - r0;  // rows from r0 on
+    const size_t off = left > 0 ? (size_t)(j0 + b * KEYS + r0) * HD + c8 * 8 : 0;
+#pragma unroll
+    for (int j = 0; j < KEYS / RS; ++j) {
+      const bool ok = j * RS < left;
+      const int step = ok ? j * RS * HD : 0, at = ap_at<HD>(r0 + j * RS, c8);  // past the end: zeros, not read
+      ap_cp16(kd + at, k + off + step, ok);
+      ap_cp16(kd + TILE + at, v + off + step, ok);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  issue(0);
+  // Q straight into A fragments: rows g and g + 8
+  uint32_t qa[HD / 16][4];
+  {
+    const __half* q = a.q + ((size_t)m * a.nh + kv * n + g) * HD + 2 * c;
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        qa[kk][x] = g + 8 * (x & 1) < n ? *reinterpret_cast<const uint32_t*>(q + (x & 1) * 8 * HD + 16 * kk + (x >> 1) * 8) : 0u;
+  }
+  float o[HD / 8][4];
+#pragma unroll
+  for (int d = 0; d < HD / 8; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  const float scale = rsqrtf((float)HD) * 1.4426950408889634f;  // scores in powers of two
+  const int lm = lane >> 3, lr = lane & 7;
+
+  for (int b = 0; b < nb; ++b) {
+    if (b + 1 < nb) {
+      issue(b + 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncwarp();
+    const __half* ks = buf + (b & 1) * 2 * TILE;
+    const __half* vs = ks + TILE;
+    float sc[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; kk += 2) {
+        uint32_t bb[4];
+        ap_ldsm4(ks + ap_at<HD>(8 * t + lr, 2 * kk + lm), bb);
+        mma_16816(sc[t], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bb[0], bb[1]);
+        mma_16816(sc[t], qa[kk + 1][0], qa[kk + 1][1], qa[kk + 1][2], qa[kk + 1][3], bb[2], bb[3]);
+      }
+    }
+    float bm0 = -INFINITY, bm1 = -INFINITY;
+    const int k0 = j0 + b * KEYS + 2 * c;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int key = k0 + 8 * t + e;
+        const bool ok = key < j1;
+        sc[t][e] = ok ? sc[t][e] * scale : -INFINITY;
+        sc[t][2 + e] = ok ? sc[t][2 + e] * scale : -INFINITY;
+        bm0 = fmaxf(bm0, sc[t][e]);
+        bm1 = fmaxf(bm1, sc[t][2 + e]);
+        if (srow != nullptr && ok) {
+          if (g < n) srow[(size_t)g * a.lds + key] = sc[t][e];
+          if (g + 8 < n) srow[(size_t)(g + 8) * a.lds + key] = sc[t][2 + e];
+        }
+      }
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+      bm0 = fmaxf(bm0, __shfl_xor_sync(0xffffffffu, bm0, x));
+      bm1 = fmaxf(bm1, __shfl_xor_sync(0xffffffffu, bm1, x));
+    }
+    const float mn0 = fmaxf(m0, bm0), mn1 = fmaxf(m1, bm1);
+    const float f0 = mn0 == -INFINITY ? 0.f : mn0 - kApShift, f1 = mn1 == -INFINITY ? 0.f : mn1 - kApShift;
+    const float al0 = ap_exp2(m0 - (mn0 == -INFINITY ? 0.f : mn0)), al1 = ap_exp2(m1 - (mn1 == -INFINITY ? 0.f : mn1));
+    m0 = mn0;
+    m1 = mn1;
+    uint32_t hi[4], lo[4] = {0u, 0u, 0u, 0u};
+    float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = (x & 1) ? f1 : f0;
+      const float p0 = ap_exp2(sc[x >> 1][2 * (x & 1)] - f), p1 = ap_exp2(sc[x >> 1][2 * (x & 1) + 1] - f);
+      if (x & 1)
+        rs1 += p0 + p1;
+      else
+        rs0 += p0 + p1;
+      const __half2 h = __floats2half2_rn(p0, p1);
+      hi[x] = h2_bits(h);
+      if (FINE) {
+        const float2 w = __half22float2(h);
+        lo[x] = h2_bits(__floats2half2_rn(p0 - w.x, p1 - w.y));
+      }
+    }
+    l0 = l0 * al0 + rs0;
+    l1 = l1 * al1 + rs1;
+    if (__any_sync(0xffffffffu, al0 != 1.f || al1 != 1.f)) {  // a maximum moved (a NaN factor counts)
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d) {
+        o[d][0] *= al0;
+        o[d][1] *= al0;
+        o[d][2] *= al1;
+        o[d][3] *= al1;
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 8; d += 2) {
+      uint32_t bb[4];
+      ap_ldsm4_t(vs + ap_at<HD>(8 * (lm & 1) + lr, d + (lm >> 1)), bb);
+      mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], bb[0], bb[1]);
+      mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], bb[2], bb[3]);
+      if (FINE) {
+        mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
+        mma_16816(o[d + 1], lo[0], lo[1], lo[2], lo[3], bb[2], bb[3]);
+      }
+    }
+    __syncwarp();  // stage b & 1 is free for block b + 2
+  }
+#pragma unroll
+  for (int x = 1; x <= 2; x <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, x);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, x);
+  }
+  const int S = a.S_p + a.S_o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = g + 8 * h;
+    if (r >= n) continue;
+    const float mx = h ? m1 : m0, l = h ? l1 : l0;
+    const size_t mh = (size_t)m * a.nh + kv * n + r;
+    if (a.direct) {
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+        *reinterpret_cast<__half2*>(a.out + mh * HD + 8 * d + 2 * c) = __floats2half2_rn(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+    } else {
+#pragma unroll
+      for (int d = 0; d < HD / 8; ++d)
+        *reinterpret_cast<float2*>(a.acc + (mh * S + split) * HD + 8 * d + 2 * c) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+      if (c == 0) a.stat[mh * S + split] = make_float2(mx, l);
+    }
+  }
+}
+
+// WRP, WRO: warps along the rows of a prefix tile and of an own tile (WRP 0: no prefix here; WRO 0:
+// own entries by single warps).
 // FINE: weights in two fp16 terms.
 template <int HD, int WRP, int WRO, bool FINE>
 __device__ __forceinline__ void ap_work(const ApArgs& a) {
@@ -342,6 +503,31 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     return;
   }
   b -= a.blocks_p;  // a range of one row's own entries for the G heads of a K/V head
+  if constexpr (WRO == 0) {
+    b = b * 4 + (int)(threadIdx.x >> 5);  // K/V heads fastest: a CTA's warps mostly share a row
+    const int kv = b % a.nkv;
+    b /= a.nkv;
+    const int split = b % a.S_o, m = b / a.S_o;
+    if (m >= a.M) return;
+    const bool first = (threadIdx.x & 31) == 0;
+    int slot, len;
+    if (!ap_row(a, m, slot, len)) {
+      if (first) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
+      return;
+    }
+    const int per = ap_range(len, a.S_o), j0 = split * per, j1 = min(len, j0 + per);
+    if (j0 >= j1) {
+      if (a.direct && len == 0)  // nothing to attend to
+        for (int i = threadIdx.x & 31; i < a.G * HD; i += 32)
+          a.out[((size_t)m * a.nh + kv * a.G) * HD + i] = __float2half_rn(0.f);
+      return;
+    }
+    const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
+    ap_warp<HD, FINE>(a, m, kv, a.kc + base, a.vc + base, j0, j1, a.S_p + split,
+                      a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr);
+    return;
+  }
+  constexpr int WR = WRO ? WRO : 1;
   const int tile = b % a.tiles_o;
   b /= a.tiles_o;
   const int split = b % a.S_o;
@@ -352,7 +538,7 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     if (threadIdx.x == 0) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
     return;
   }
-  constexpr int tr = 16 * WRO;
+  constexpr int tr = 16 * WR;
   const int i0 = tile * tr, n = min(tr, a.G - i0);
   const int per = ap_range(len, a.S_o), j0 = split * per, j1 = min(len, j0 + per);
   if (j0 >= j1) {
@@ -363,7 +549,7 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
   float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile<HD, WRO, FINE>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
+  ap_tile<HD, WR, FINE>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
                  a.S_p + split);
 }
 
@@ -625,7 +811,7 @@ __global__ void __launch_bounds__(128) attn_prefix_join_kernel(const ApArgs a, i
 
 // How a call is cut: rows per tile, key ranges, workspace. The same for the size query.
 struct ApPlan {
-  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, blk_p, tr_p, tc, row, direct, lds;
+  int G, wr_p, wr_o, tiles_p, tiles_o, S_p, S_o, blk_p, tr_p, tc, row, by_warp, direct, lds;
   size_t acc_floats, stat_floats, score_floats;
   size_t bytes() const { return (acc_floats + stat_floats + score_floats) * sizeof(float); }
 };
@@ -636,6 +822,7 @@ constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V head
 // 2,048 entries (128 blocks) 16.5 us with them, 12.0 without; 64 x 32 heads behind 512 (128 blocks)
 // 25.2 and 24.7, behind 1,024 26.1 and 28.0, behind 4,096 65.8 and 80.
 constexpr int kApTcFrom = 32, kApTcBlocks = 256;
+constexpr uint32_t kApWarpKeys = 256;  // own entries of a row up to which single warps take them
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
@@ -684,7 +871,9 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
     p.S_p = ranges(items, max_prefix, items * (max_prefix / 256) >= (size_t)num_sms() / 2 ? 256 : 128);
   }
   const size_t own_items = (size_t)M * nkv * p.tiles_o;
-  p.S_o = ranges(own_items, max_own, own_items >= (size_t)num_sms() ? 128 : 64);
+  p.by_warp = p.G <= 16 && max_own <= kApWarpKeys && own_items >= 2 * (size_t)num_sms();
+  p.S_o = p.by_warp ? (int)std::max<size_t>(1, std::min<size_t>((12 * (size_t)num_sms() + own_items - 1) / own_items, max_own / 128))
+                    : ranges(own_items, max_own, own_items >= (size_t)num_sms() ? 128 : 64);
   // Few CTAs with little to read: splitting would cost a second launch and more than it saves (2 x
   // 2 heads of 32 keys: 3.2 us in one launch, 4.9 in two; one row of 32 heads x 577 keys, tracked:
   // 15.9 and 9.7). Weights only for a single row: rows that share a slot need an order.
@@ -710,12 +899,12 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
   const int dev = device_index();
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
     ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD, WRP, WRO, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD, WRO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD, WRO ? WRO : 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_done[dev] = true;
   }
   const dim3 none(0, 0, 0);
   if (a.row) {
-    ORCH_CUDA(launch_k_serial(attn_prefix_row_kernel<HD, WRO>, dim3((unsigned)(a.M * a.nkv * a.tiles_o)), dim3(128), smem,
+    ORCH_CUDA(launch_k_serial(attn_prefix_row_kernel<HD, WRO ? WRO : 1>, dim3((unsigned)(a.M * a.nkv * a.tiles_o)), dim3(128), smem,
                               st, none, a));
     return check_launch("attention_prefix");
   }
@@ -724,7 +913,7 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
     if (rc != ORCH_OK) return rc;
     a.blocks_p = 0;
   }
-  const size_t blocks = (size_t)a.blocks_p + (size_t)a.M * a.nkv * a.S_o * a.tiles_o;
+  const size_t own = (size_t)a.M * a.nkv * a.S_o * a.tiles_o, blocks = (size_t)a.blocks_p + (WRO ? own : (own + 3) / 4);
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
   ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO, FINE>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
   if (a.direct) return check_launch("attention_prefix");
@@ -747,13 +936,17 @@ int ap_launch_wr(const ApArgs& a, cudaStream_t st) {
 template <int HD>
 int ap_launch(const ApArgs& a, cudaStream_t st) {
   const int p = a.tc || a.row || a.blocks_p == 0 ? 0 : a.wr_p;
+  const int o = a.by_warp ? 0 : a.wr_o;
   if (p == 0)
-    return a.wr_o == 1 ? ap_launch_wr<HD, 0, 1>(a, st) : a.wr_o == 2 ? ap_launch_wr<HD, 0, 2>(a, st) : ap_launch_wr<HD, 0, 4>(a, st);
-  if (p == 1) return ap_launch_wr<HD, 1, 1>(a, st);
-  if (p == 2) return a.wr_o == 1 ? ap_launch_wr<HD, 2, 1>(a, st) : ap_launch_wr<HD, 2, 2>(a, st);
+    return o == 0 ? ap_launch_wr<HD, 0, 0>(a, st) : o == 1 ? ap_launch_wr<HD, 0, 1>(a, st)
+         : o == 2 ? ap_launch_wr<HD, 0, 2>(a, st) : ap_launch_wr<HD, 0, 4>(a, st);
+  if (p == 1) return o == 0 ? ap_launch_wr<HD, 1, 0>(a, st) : ap_launch_wr<HD, 1, 1>(a, st);
+  if (p == 2)
+    return o == 0 ? ap_launch_wr<HD, 2, 0>(a, st) : o == 1 ? ap_launch_wr<HD, 2, 1>(a, st) : ap_launch_wr<HD, 2, 2>(a, st);
   if constexpr (HD == 32) {
-    if (a.wr_o == 1) return ap_launch_wr<HD, 4, 1>(a, st);
-    if (a.wr_o == 2) return ap_launch_wr<HD, 4, 2>(a, st);
+    if (o == 0) return ap_launch_wr<HD, 4, 0>(a, st);
+    if (o == 1) return ap_launch_wr<HD, 4, 1>(a, st);
+    if (o == 2) return ap_launch_wr<HD, 4, 2>(a, st);
   }
   return ap_launch_wr<HD, 4, 4>(a, st);
 }
@@ -842,6 +1035,7 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.blocks_p = (int)blocks_p;
   a.direct = p.direct;
   a.row = p.row;
+  a.by_warp = p.by_warp;
   a.fine = (uint64_t)M * num_kv_heads <= kApDirectPairs;
   a.acc = static_cast<float*>(workspace);
   a.stat = reinterpret_cast<float2*>(a.acc + p.acc_floats);

@@ -34,6 +34,7 @@ struct ApArgs {
   int tc;                // the prefix part runs in its own kernel (attention_prefix_tc.cu)
   int blocks_p;          // CTAs of the prefix part (the first ones of the grid)
   int row;               // few rows and keys: a CTA per row and K/V head takes all of them
+  int by_warp;           // own entries by single warps, four rows and K/V heads per CTA
   int fine;              // weights in two fp16 terms
   int direct;            // the output is written by the attention kernel: nothing to join
   float* acc;            // [M * nh][S][HD]

@@ -627,3 +627,23 @@ def test_logits_long_lists(H, nb):
             want[v] += b
         assert np.all(np.abs(got[m] - want) <= 2.0 ** -22 * (np.abs(want) + np.abs(x[m]) + 100))
     assert flags() == 0
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("hd,nh,nkv,rows,plen,cap", [(128, 32, 32, 12, 0, 70), (64, 64, 8, 45, 90, 256), (32, 48, 16, 21, 200, 17),
+                                                     (128, 48, 3, 101, 33, 130), (64, 7, 7, 50, 900, 256)])
+def test_many_rows_with_short_entries(hd, nh, nkv, rows, plen, cap, track):
+    """Enough rows and K/V heads that single warps take the own entries (up to 256 of them), with
+    and without a prefix beside them, empty and rejected rows among them."""
+    lens = [(i * 37) % (cap + 1) for i in range(rows)]
+    host = case(rows + hd, hd, nh, nkv, [(0, rows - 1, 0, plen)] if plen else [], lens, cap, nslots=rows + 2, pcap=max(plen, 1))
+    mass = rng(4, rows).random((rows + 2, nkv, cap), dtype=np.float32) if track else None
+    got = check_attention(host, mass)
+    q, kp, vp, units, kc, vc, n, slots = host
+    n, slots = n.copy(), slots.copy()
+    n[3], slots[5] = cap + 1, -1
+    dm = D(mass) if track else None
+    out = attention(D(q), D(kp), D(vp), D(units) if len(units) else None, D(kc), D(vc), D(n), D(slots), dm)
+    assert flags() == 2 | 8 and (out[[3, 5]] == 7).all()
+    ok = [i for i in range(rows) if i not in (3, 5)]
+    assert torch.equal(out[ok], got[ok])
