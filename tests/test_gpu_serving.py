@@ -502,14 +502,18 @@ def bits(allowed, words):
 
 
 def run_logits(x, base=0, ld=None, hist=None, hist_len=None, gen=None, pen=None, bias=None, masks=None, mask_rows=None,
-               inplace=False):
-    """x: host [M, V]; bias: per row lists of (id, value)."""
+               inplace=False, shift=(0, 0)):
+    """x: host [M, V]; bias: per row lists of (id, value); shift: elements that in and out begin
+    past an aligned place."""
     M, V = x.shape
     ld = ld or V
     buf = np.full((M, ld), 3.0, x.dtype)
     buf[:, :V] = x
-    din = D(buf)
-    dout = din if inplace else torch.full_like(din, 9.0)
+    room = torch.full((M * ld + 64,), 5.0, dtype=D(buf).dtype, device="cuda")
+    room2 = torch.full_like(room, 5.0)
+    din = room[shift[0]:shift[0] + M * ld].view(M, ld)
+    din.copy_(D(buf))
+    dout = din if inplace else room2[shift[1]:shift[1] + M * ld].view(M, ld).fill_(9.0)
     ids = vals = off = None
     nb = 0
     if bias is not None:
@@ -523,13 +527,15 @@ def run_logits(x, base=0, ld=None, hist=None, hist_len=None, gen=None, pen=None,
          None if masks is None else D(masks.view(np.int32)), 0 if masks is None else masks.shape[1],
          0 if masks is None else masks.shape[0], None if mask_rows is None else D(mask_rows), S())
     out = dout.cpu().numpy()
+    for r, k in ((room, shift[0]), (room2, shift[0] if inplace else shift[1])):  # nothing around them is touched
+        assert (r[:k] == 5).all() and (r[k + M * ld:] == 5).all()
     assert (out[:, V:] == (3.0 if inplace else 9.0)).all()  # columns between rows are not touched
     return out[:, :V]
 
 
 @pytest.mark.parametrize("dt", [np.float32, np.float16])
 @pytest.mark.parametrize("V,M,base,pad", [(1, 2, 0, 0), (31, 3, 0, 1), (64, 1, 40, 0), (1000, 5, 17, 3), (32000, 2, 0, 0),
-                                          (9001, 4, 12345, 2)])
+                                          (9001, 4, 12345, 2), (2047, 6, 0, 0), (2049, 3, 32, 1)])
 def test_logits(V, M, base, pad, dt):
     g = rng(7, V, M)
     x = (3 * g.standard_normal((M, V), dtype=np.float32)).astype(dt)
@@ -547,8 +553,8 @@ def test_logits(V, M, base, pad, dt):
     allow = [set(int(v) for v in g.integers(base, base + V, V // 3 + 1)), set(), set(range(base + V))]
     masks = np.stack([bits(a, words) for a in allow])
     mask_rows = np.array([(-1, 0, 2, 1)[i % 4] for i in range(M)], np.int32)
-    for inplace in (False, True):
-        got = run_logits(x, base, V + pad, hist, hist_len, gen, pen, bias, masks, mask_rows, inplace)
+    for inplace, shift in ((False, (0, 0)), (True, (0, 0)), (False, (1, 1)), (True, (3, 3)), (False, (7, 7)), (False, (2, 5))):
+        got = run_logits(x, base, V + pad, hist, hist_len, gen, pen, bias, masks, mask_rows, inplace, shift)
         for m in range(M):
             want = serving.logits_process(x[m], base, hist[m, :hist_len[m]], int(gen[m]), pen[m],
                                           [(v, np.float32(w)) for v, w in bias[m]],

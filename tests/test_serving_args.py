@@ -53,7 +53,7 @@ def test_evict_refusals(kw, word):
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(x=None), b"null"), (dict(out=None), b"null"), (dict(V=0), b"empty"), (dict(dt=2), b"dtype"), (dict(ld=9), b"stride"),
+    (dict(x=None), b"null"), (dict(out=None), b"null"), (dict(V=0), b"empty"), (dict(dt=2), b"dtype"), (dict(ld=9), b"stride"), (dict(ld=1 << 31), b"stride"),
     (dict(base=2 ** 31 - 5), b"range"), (dict(hist=P), b"penalties"), (dict(pen=P), b"penalties"), (dict(hist=P, pen=P), b"penalties"),
     (dict(bi=P), b"bias"), (dict(bi=P, bv=P), b"bias"), (dict(masks=P, mw=1, nm=1), b"masks"), (dict(masks=P, mr=P), b"masks"),
     (dict(M=65536), b"rows")])
