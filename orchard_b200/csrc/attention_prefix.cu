@@ -822,7 +822,11 @@ constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V head
 // 2,048 entries (128 blocks) 16.5 us with them, 12.0 without; 64 x 32 heads behind 512 (128 blocks)
 // 25.2 and 24.7, behind 1,024 26.1 and 28.0, behind 4,096 65.8 and 80.
 constexpr int kApTcFrom = 32, kApTcBlocks = 256;
-constexpr uint32_t kApWarpKeys = 256;  // own entries of a row up to which single warps take them
+// Own entries of a row up to which single warps take them, where their warps (two per SM or more)
+// fill the SMs, and up to which they always do. 64 x 32 heads of up to 64, 128 and 256 entries: 14.1,
+// 20.6 and 35.8 us by warps, 22.0, 26.5 and 35.8 by tiles; 4 x 8 heads x 4 of up to 256: 11.2 and
+// 8.2; 32 x 8 heads x 4 of up to 64: 10.1 and 10.9.
+constexpr uint32_t kApWarpKeys = 256, kApWarpAlways = 64;
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 
@@ -871,7 +875,7 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
     p.S_p = ranges(items, max_prefix, items * (max_prefix / 256) >= (size_t)num_sms() / 2 ? 256 : 128);
   }
   const size_t own_items = (size_t)M * nkv * p.tiles_o;
-  p.by_warp = p.G <= 16 && max_own <= kApWarpKeys && own_items >= 2 * (size_t)num_sms();
+  p.by_warp = p.G <= 16 && max_own <= (own_items >= 2 * (size_t)num_sms() ? kApWarpKeys : kApWarpAlways);
   p.S_o = p.by_warp ? (int)std::max<size_t>(1, std::min<size_t>((12 * (size_t)num_sms() + own_items - 1) / own_items, max_own / 128))
                     : ranges(own_items, max_own, own_items >= (size_t)num_sms() ? 128 : 64);
   // Few CTAs with little to read: splitting would cost a second launch and more than it saves (2 x
