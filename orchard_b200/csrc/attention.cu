@@ -512,14 +512,16 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const float* logits, 
   const float before = wprefix + incl - local;  // sum of all earlier chunks
   const float target = uniforms[blockIdx.x] * total;
   if (local > 0.f && before <= target && target < before + local) {
+    // Added one by one the weights may end at or below a target that lies below their sum: the
+    // last token that has a weight is then the one (one of no weight may be forbidden, its logit
+    // -inf). `local` is positive, so there is one.
     float run = before;
     int pick = c1 - 1;
     for (int i = c0; i < c1; ++i) {
-      run += expf((r[i] - mx) / temperature);
-      if (run > target) {
-        pick = i;
-        break;
-      }
+      const float e = expf((r[i] - mx) / temperature);
+      run += e;
+      if (e > 0.f) pick = i;
+      if (run > target) break;
     }
     if (atomicCAS(&found, 0, 1) == 0) tok[blockIdx.x] = pick;
   }
