@@ -162,10 +162,10 @@ class RowControls:
             self.mask_rows.fill_(-1)
             return
         m = np.ascontiguousarray(masks, np.uint32)
-        if m.ndim != 2 or m.shape[0] > self.masks.shape[0] or m.shape[1] != self.words:
-            raise ValueError(f"grammar masks must be [rows, {self.words}] words")
-        self.masks[:m.shape[0]].copy_(torch.from_numpy(m.view(np.int32)))
-        self.mask_rows[:m.shape[0]].copy_(torch.arange(m.shape[0], dtype=torch.int32))
+        if m.shape != tuple(self.masks.shape):  # fewer rows would leave the others an earlier step's masks
+            raise ValueError(f"grammar masks must be [{self.masks.shape[0]} rows, {self.words} words]")
+        self.masks.copy_(torch.from_numpy(m.view(np.int32)))
+        self.mask_rows.copy_(torch.arange(m.shape[0], dtype=torch.int32))
 
     def apply(self, logits: torch.Tensor, M: int, V: int):
         pen = self.penal
