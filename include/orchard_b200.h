@@ -59,7 +59,8 @@ int orch_device_name(char* buf, size_t len);
  * or a bad prefill unit (its output not written); 4 an embedding id outside the vocabulary
  * (zero row); 8 a cache slot outside [0, num_slots) (no cache read or write for that row);
  * 16 a row of orch_logits_process whose history length, bias range or mask index lies
- * outside what the call was given (that row not written);
+ * outside what the call was given (that row not written); 32 a row of orch_argmax_rows or
+ * orch_sample_rows whose logits are all -inf (no token left to choose: its token is 0);
  * 256 a tensor-core GEMM's bounded wait ran out; 512 a peer all-reduce's wait for another
  * rank ran out. Covers the allocation-free attention entry point's flags as well. */
 int orch_device_check(uint32_t* flags_out, void* stream);

@@ -315,7 +315,7 @@ __device__ __forceinline__ bool argmax_better(float v, int i, float best, int bi
 // PAIRS: also write the row's maximum (as float) and base + index (as float, exact below
 // 2^24) to out_pairs[row] for the vocabulary-split merge.
 template <bool PAIRS>
-__global__ void argmax_rows_kernel(const float* logits, int V, int* out, float2* out_pairs, int base) {
+__global__ void argmax_rows_kernel(const float* logits, int V, int* out, float2* out_pairs, int base, uint32_t* check) {
   __shared__ float sv[32];
   __shared__ int si[32];
   pdl_trigger();
@@ -377,10 +377,12 @@ __global__ void argmax_rows_kernel(const float* logits, int V, int* out, float2*
     }
     if (lane == 0) {
       const int i = bi == 0x7fffffff ? 0 : bi;
-      if (PAIRS)
+      if (PAIRS) {
         out_pairs[blockIdx.x] = make_float2(best, (float)(base + i));
-      else
+      } else {
         out[blockIdx.x] = i;
+        if (best == -INFINITY && check != nullptr) atomicOr(check, 32u);  // no token left to choose
+      }
     }
   }
 }
@@ -458,7 +460,7 @@ extern "C" int orch_argmax_rows(const float* logits, uint32_t M, uint32_t V, int
   if (M == 0) return ORCH_OK;
   ORCH_REQUIRE(logits && out && V > 0, "argmax_rows: bad arguments");
   ORCH_CUDA(launch_k(argmax_rows_kernel<false>, dim3(M), dim3(1024), 0, as_stream(stream), dim3(0, 0, 0), logits,
-                     (int)V, (int*)out, (float2*)nullptr, 0));
+                     (int)V, (int*)out, (float2*)nullptr, 0, device_check_word()));
   return check_launch("argmax_rows");
 }
 
@@ -468,7 +470,7 @@ extern "C" int orch_argmax_pairs(const float* logits, uint32_t M, uint32_t V, ui
   if (M == 0) return ORCH_OK;
   ORCH_REQUIRE(logits && pairs && V > 0 && base + V < (1u << 24), "argmax_pairs: bad arguments");
   ORCH_CUDA(launch_k(argmax_rows_kernel<true>, dim3(M), dim3(1024), 0, as_stream(stream), dim3(0, 0, 0), logits,
-                     (int)V, (int*)nullptr, (float2*)pairs, (int)base));
+                     (int)V, (int*)nullptr, (float2*)pairs, (int)base, (uint32_t*)nullptr));
   return check_launch("argmax_pairs");
 }
 
@@ -479,7 +481,7 @@ namespace orch {
 // thread owns a contiguous chunk; chunk sums are scanned across the block, and the thread
 // whose chunk holds the crossing walks it in order.
 __global__ void __launch_bounds__(1024) sample_rows_kernel(const float* logits, int V, float temperature,
-                                                           const float* uniforms, int* tok) {
+                                                           const float* uniforms, int* tok, uint32_t* check) {
   __shared__ float red[32];
   __shared__ float wsum[32];
   __shared__ int found;
@@ -489,6 +491,12 @@ __global__ void __launch_bounds__(1024) sample_rows_kernel(const float* logits, 
   float mx = -INFINITY;
   for (int i = threadIdx.x; i < V; i += blockDim.x) mx = fmaxf(mx, r[i]);
   mx = block_max(mx, red);
+  if (mx == -INFINITY) {  // no token left to choose, unless there are NaNs; token 0 is taken below
+    int nan = 0;
+    for (int i = threadIdx.x; i < V; i += blockDim.x) nan |= r[i] != r[i];
+    nan = __syncthreads_or(nan);
+    if (threadIdx.x == 0 && !nan && check != nullptr) atomicOr(check, 32u);
+  }
   const int chunk = (V + blockDim.x - 1) / blockDim.x;
   const int c0 = min(V, (int)threadIdx.x * chunk), c1 = min(V, c0 + chunk);
   float local = 0.f;
@@ -560,7 +568,7 @@ extern "C" int orch_sample_rows(const float* logits, uint32_t M, uint32_t V, flo
   ORCH_REQUIRE(logits && uniforms && tok && V > 0, "sample_rows: bad arguments");
   ORCH_REQUIRE(temperature > 0.f, "sample_rows: temperature must be positive (0 is argmax)");
   ORCH_CUDA(launch_k(sample_rows_kernel, dim3(M), dim3(1024), 0, as_stream(stream), dim3(0, 0, 0), logits, (int)V,
-                     temperature, uniforms, (int*)tok));
+                     temperature, uniforms, (int*)tok, device_check_word()));
   return check_launch("sample_rows");
 }
 

@@ -38,7 +38,8 @@ class LogitsControls:
     occurrence for tokens of the answer. ``bias`` maps token ids to additions. ``allowed(step,
     answers)`` returns the step's grammar masks, uint32 ``[rows, ceil(vocab / 32)]`` (bit v & 31
     of word v >> 5 set: token v allowed), or None for no restriction; it is given the answers so
-    far, so with it every step waits for the one before."""
+    far, so with it every step waits for the one before. A mask has to leave every row that still
+    answers a token; those of rows that have ended are not looked at."""
 
     repetition: float = 1.0
     presence: float = 0.0
@@ -152,20 +153,27 @@ class RowControls:
         self.bias_ids = torch.as_tensor(np.tile(ids, rows)).to(device)
         self.bias_vals = torch.as_tensor(np.tile(np.asarray(list(c.bias.values()), np.float32), rows)).to(device)
         self.bias_off = torch.arange(0, rows + 1, **i32) * len(ids)
-        self.words = (vocab + 31) // 32
+        self.vocab, self.words = vocab, (vocab + 31) // 32
         self.masks = torch.zeros((rows, self.words), **i32) if c.allowed is not None else None
         self.mask_rows = torch.full((rows,), -1, **i32)
 
-    def set_masks(self, masks: Optional[np.ndarray]):
-        """The next step's masks, one per row (None: every token allowed)."""
+    def set_masks(self, masks: Optional[np.ndarray], active: Optional[np.ndarray] = None):
+        """The next step's masks, one per row (None: every token allowed); ``active`` (None: all)
+        says which rows still answer."""
         if masks is None:
             self.mask_rows.fill_(-1)
             return
         m = np.ascontiguousarray(masks, np.uint32)
         if m.shape != tuple(self.masks.shape):  # fewer rows would leave the others an earlier step's masks
             raise ValueError(f"grammar masks must be [{self.masks.shape[0]} rows, {self.words} words]")
+        active = np.ones(len(m), bool) if active is None else np.asarray(active, bool)
+        left = m.any(axis=1)
+        if self.vocab % 32:  # bits past the vocabulary do not count
+            left = m[:, :-1].any(axis=1) | (m[:, -1] & np.uint32((1 << self.vocab % 32) - 1) != 0)
+        if (active & ~left).any():
+            raise ValueError(f"the grammar mask of row {int(np.argmax(active & ~left))} allows no token")
         self.masks.copy_(torch.from_numpy(m.view(np.int32)))
-        self.mask_rows.copy_(torch.arange(m.shape[0], dtype=torch.int32))
+        self.mask_rows.copy_(torch.from_numpy(np.where(active, np.arange(len(m)), -1).astype(np.int32)))
 
     def apply(self, logits: torch.Tensor, M: int, V: int):
         pen = self.penal
@@ -307,7 +315,7 @@ class BatchServer:
             index.copy_(up[1])
             n_own.copy_(up[2])
             if controls is not None and controls.allowed is not None:
-                rc.set_masks(controls.allowed(s, gen))
+                rc.set_masks(controls.allowed(s, gen), active)
             if temperature > 0:  # one uniform per active row, in row order
                 u = np.full(B, 0.5, np.float32)
                 u[active] = np.random.random_sample(int(active.sum()))
@@ -336,5 +344,6 @@ class BatchServer:
         flags = _lib.C.c_uint32(0)
         call("orch_device_check", _lib.C.byref(flags), _stream())
         if flags.value:
-            raise RuntimeError(f"a kernel rejected its input (device check bits {flags.value})")
+            raise RuntimeError(("the controls left a row no token (device check bit 32)" if flags.value == 32 else
+                                f"a kernel rejected its input (device check bits {flags.value})"))
         return gen

@@ -86,3 +86,22 @@ def test_draws_under_a_mask_are_allowed_tokens(T):
     got = sample(masked(x, allowed), T, u)
     assert all(got[m] in allowed[m] for m in range(M))
     assert flags() == 0
+
+
+def test_a_row_without_any_token_is_reported():
+    """All -inf: token 0 and device check bit 32, greedy and drawn; other rows are not affected."""
+    V = 1000
+    x = np.tile(np.linspace(-1, 1, V, dtype=np.float32), (4, 1))
+    lg = masked(x, [[5, 9], [], [V - 1], []])
+    tok = torch.full((4,), -7, dtype=torch.int32, device="cuda")
+    call("orch_argmax_rows", lg, 4, V, tok, S())
+    assert flags() == 32 and tok.tolist() == [9, 0, V - 1, 0]
+    assert sample(lg, 0.7, [0.0, 0.5, 0.9, 0.1]).tolist() == [5, 0, V - 1, 0]
+    assert flags() == 32
+    lg = masked(x, [[5, 9], [7], [V - 1], [0]])
+    call("orch_argmax_rows", lg, 4, V, tok, S())
+    sample(lg, 0.7, [0.0, 0.5, 0.9, 0.1])
+    assert flags() == 0
+    lg[1] = float("nan")  # a NaN is a value as before
+    call("orch_argmax_rows", lg, 4, V, tok, S())
+    assert flags() == 0 and tok[1] == 0
