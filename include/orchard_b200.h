@@ -314,8 +314,9 @@ int orch_embed_rows(const int32_t* ids, const void* table, int table_dt, float* 
  * entry received, summed over the query heads of its K/V head: added to entries below
  * lens[m] - 1, stored into entry lens[m] - 1 (the newest: it has no earlier weight). Rows that
  * share a slot are taken in row order; sums have one order, so results repeat bit for bit.
- * A row whose slot or length is out of range, or whose unit is, is not written (nor its mass)
- * and sets device check bit 8 (slot) / 2. `workspace`, 16-byte aligned, holds
+ * A row whose slot or length is out of range, whose unit is, or that is in two units, is not
+ * written (nor its mass) and sets device check bit 8 (slot) / 2; where units overlap, so may be
+ * rows of the units after them. `workspace`, 16-byte aligned, holds
  * orch_attention_prefix_workspace_bytes() bytes (the same arguments; track: mass given). */
 size_t orch_attention_prefix_workspace_bytes(uint32_t M, uint32_t num_heads, uint32_t num_kv_heads,
                                              uint32_t head_dim, uint32_t num_units, uint32_t max_prefix,

@@ -482,6 +482,13 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
 template <int HD, int WRP, int WRO, bool FINE>
 __device__ __forceinline__ void ap_work(const ApArgs& a) {
   int b = blockIdx.x;
+  if (a.num_units > 0) {  // the first CTA reports the rejected units
+    if (b == 0) {
+      ap_report_units(a);
+      return;
+    }
+    --b;
+  }
   if (WRP > 0 && b < a.blocks_p) {  // a range of a prefix for a tile of the unit's query rows
     // row tiles fastest: the tiles that read the same keys run together
     const int tile = b % a.tiles_p;
@@ -490,10 +497,6 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     int4 u;
     const int i0 = ap_find_tile(a, tile, u);
     if (i0 < 0) return;
-    if (!ap_unit_ok(a, u)) {
-      if (threadIdx.x == 0) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
-      return;
-    }
     const int n = min(a.tr_p, u.y * a.G - i0);
     const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
     if (j0 >= j1) return;
@@ -558,21 +561,24 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
   pdl_trigger();
   // Beside the prefix's own kernel, launched just before: that kernel waited for everything
   // earlier before it let this one start, and the two share no output, so they run together.
-  // One CTA stays until it has ended, so that whoever waits for this grid waits for both.
+  // The first CTA stays until it has ended, so that whoever waits for this grid waits for both.
   if (!a.tc) pdl_wait();
   ap_work<HD, WRP, WRO, FINE>(a);
   if (a.tc && blockIdx.x == 0) pdl_wait();
 }
 
-// The prefix of row m: its slot and length (0: none). False when the row's unit was rejected or
-// the row is in two. (Called by whole warps.)
+// The prefix of row m: its slot and length (0: none). False when the row's unit was rejected, the
+// row is in two, or (TILES) overlapping units left its tile no CTA. (Called by whole warps.)
+template <bool TILES>
 __device__ __forceinline__ bool ap_row_prefix(const ApArgs& a, int m, int& pslot, int& plen) {
+  constexpr int kMany = 1 << 26;
   const int lane = threadIdx.x & 31;
-  int bad = 0, in = 0, z = 0, w = 0;
+  int bad = 0, in = 0, z = 0, w = 0, tiles = 0;
   for (int u0 = 0; u0 < a.num_units; u0 += 32) {
     const int i = u0 + lane;
     if (i < a.num_units) {
       const int4 u = a.units[i];
+      if (TILES) tiles = min(tiles + ap_unit_tiles(a, u), kMany);
       if (m >= u.x && (long long)m < (long long)u.x + u.y) {
         if (ap_unit_ok(a, u)) {
           z = u.z, w = u.w;
@@ -587,7 +593,13 @@ __device__ __forceinline__ bool ap_row_prefix(const ApArgs& a, int m, int& pslot
   if (in > 1 && lane == 0) atomicOr(a.check, 2u);
   pslot = (int)__reduce_add_sync(0xffffffffu, (unsigned)z);  // one lane's at most, when in <= 1
   plen = (int)__reduce_add_sync(0xffffffffu, (unsigned)w);
-  return !__any_sync(0xffffffffu, bad) && in <= 1;
+  if (__any_sync(0xffffffffu, bad) || in > 1) return false;
+  if (TILES && (__reduce_add_sync(0xffffffffu, (unsigned)tiles) > (unsigned)a.tiles_p || __any_sync(0xffffffffu, tiles == kMany)) &&
+      !ap_row_has_tile(a, m)) {
+    if (lane == 0) atomicOr(a.check, 2u);
+    return false;
+  }
+  return true;
 }
 
 // Ranges of row m that hold keys: prefix ranges 0 .. np - 1, own ranges S_p .. S_p + no - 1.
@@ -595,7 +607,7 @@ __device__ __forceinline__ bool ap_row_prefix(const ApArgs& a, int m, int& pslot
 __device__ __forceinline__ bool ap_ranges(const ApArgs& a, int m, int& slot, int& len, int& np, int& no) {
   int pslot, plen;
   const bool ok = ap_row(a, m, slot, len);
-  if (!ap_row_prefix(a, m, pslot, plen) || !ok) return false;
+  if (!ap_row_prefix<true>(a, m, pslot, plen) || !ok) return false;
   np = plen > 0 ? (plen + ap_range(plen, a.S_p, a.blk_p) - 1) / ap_range(plen, a.S_p, a.blk_p) : 0;
   no = len > 0 ? (len + ap_range(len, a.S_o) - 1) / ap_range(len, a.S_o) : 0;
   return true;
@@ -608,15 +620,11 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a)
   pdl_trigger();
   pdl_wait();
   const int tile = blockIdx.x % a.tiles_o, b = blockIdx.x / a.tiles_o, kv = b % a.nkv, m = b / a.nkv;
-  if (blockIdx.x == 0)  // units are reported once, whether or not a row is in them
-    for (int i = threadIdx.x; i < a.num_units; i += 128) {
-      const int4 u = a.units[i];
-      if (!ap_unit_ok(a, u)) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
-    }
+  if (blockIdx.x == 0) ap_report_units(a);  // once, whether or not a row is in them
   int slot, len, pslot, plen;
   const bool row = ap_row(a, m, slot, len);
   if (!row && threadIdx.x == 0) atomicOr(a.check, slot < 0 || slot >= a.num_slots ? 8u : 2u);
-  if (!ap_row_prefix(a, m, pslot, plen) || !row) return;
+  if (!ap_row_prefix<false>(a, m, pslot, plen) || !row) return;
   constexpr int tr = 16 * WRO;
   const int i0 = tile * tr, n = min(tr, a.G - i0);
   if (plen + len == 0) {  // nothing to attend to
@@ -842,7 +850,8 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.wr_p = std::min(ap_wr(rows_p), hd == 32 || p.G > 32 ? 4 : 2);  // 64 rows of 64 or 128 dims spill
   p.wr_o = ap_wr(p.G);
   p.tr_p = !p.tc ? 16 * p.wr_p : rows_p > kApTcRows ? 2 * kApTcRows : kApTcRows;
-  // the units share out at most M rows: their tiles are at most this many, and about `likely`
+  // Units that share out at most M rows have at most this many tiles, and about `likely`; where
+  // they overlap they may have more, and rows past these tiles are rejected (ap_row_has_tile).
   const size_t q_rows = (size_t)M * p.G;
   p.tiles_p = some ? (int)std::min<size_t>((q_rows + (size_t)num_units * (p.tr_p - 1)) / p.tr_p, 0x7fffffff) : 0;
   const size_t likely = std::max<size_t>((q_rows + p.tr_p - 1) / p.tr_p, num_units);
@@ -917,7 +926,7 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
     if (rc != ORCH_OK) return rc;
     a.blocks_p = 0;
   }
-  const size_t own = (size_t)a.M * a.nkv * a.S_o * a.tiles_o, blocks = (size_t)a.blocks_p + (WRO ? own : (own + 3) / 4);
+  const size_t own = (size_t)a.M * a.nkv * a.S_o * a.tiles_o, blocks = (size_t)a.blocks_p + (WRO ? own : (own + 3) / 4) + (a.num_units > 0);
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
   ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO, FINE>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
   if (a.direct) return check_launch("attention_prefix");
@@ -1030,6 +1039,8 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.S_p = p.S_p;
   a.blk_p = p.blk_p;
   a.tr_p = p.tr_p;
+  for (a.tr_sh = 0; 1 << a.tr_sh < p.tr_p; ++a.tr_sh) {
+  }
   a.tc = p.tc;
   a.S_o = p.S_o;
   const uint64_t blocks_p = (uint64_t)num_kv_heads * p.tiles_p * p.S_p;

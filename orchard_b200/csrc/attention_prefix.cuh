@@ -27,12 +27,12 @@ struct ApArgs {
   __half* out;
   int M, nh, nkv, G;
   int wr_p, wr_o;        // warps along the rows of a prefix tile / an own tile
-  int tr_p;              // query rows of a prefix tile
-  int tiles_p, tiles_o;  // row tiles of all units (as many as there can be) / per row
+  int tr_p, tr_sh;       // query rows of a prefix tile, and their logarithm
+  int tiles_p, tiles_o;  // row tiles of all units (as many as disjoint ones can have) / per row
   int S_p, S_o;          // key ranges of a prefix / of a row's own entries
   int blk_p;             // keys that a range of a prefix is a multiple of
   int tc;                // the prefix part runs in its own kernel (attention_prefix_tc.cu)
-  int blocks_p;          // CTAs of the prefix part (the first ones of the grid)
+  int blocks_p;          // CTAs of the prefix part
   int row;               // few rows and keys: a CTA per row and K/V head takes all of them
   int by_warp;           // own entries by single warps, four rows and K/V heads per CTA
   int fine;              // weights in two fp16 terms
@@ -61,8 +61,19 @@ __device__ __forceinline__ bool ap_unit_ok(const ApArgs& a, const int4& u) {
   return u.y >= 1 && u.y <= kApMaxUnitRows && u.x >= 0 && u.x < a.M && u.y <= a.M - u.x && u.w >= 0 &&
          u.w <= a.max_prefix && u.z >= 0 && u.z < a.num_prefix;
 }
+// Row tiles of a unit; a rejected one has none.
+__device__ __forceinline__ int ap_unit_tiles(const ApArgs& a, const int4& u) {
+  return ap_unit_ok(a, u) ? (u.y * a.G + a.tr_p - 1) >> a.tr_sh : 0;
+}
+// Reports the rejected units. Whole CTAs call.
+__device__ __forceinline__ void ap_report_units(const ApArgs& a) {
+  for (int i = threadIdx.x; i < a.num_units; i += blockDim.x) {
+    const int4 u = a.units[i];
+    if (!ap_unit_ok(a, u)) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
+  }
+}
 // Row tile t of all units, in their order: its unit (in u) and its first query row, or -1 past
-// the last tile. A rejected unit has one tile, whose CTA reports it. Whole CTAs call.
+// the last tile. Whole warps call.
 __device__ __forceinline__ int ap_find_tile(const ApArgs& a, int t, int4& u) {
   const int lane = threadIdx.x & 31;
   for (int u0 = 0; u0 < a.num_units; u0 += 32) {
@@ -70,7 +81,7 @@ __device__ __forceinline__ int ap_find_tile(const ApArgs& a, int t, int4& u) {
     int tiles = 0;
     if (u0 + lane < a.num_units) {
       v = a.units[u0 + lane];
-      tiles = ap_unit_ok(a, v) ? (v.y * a.G + a.tr_p - 1) / a.tr_p : 1;
+      tiles = ap_unit_tiles(a, v);
     }
     int end = tiles;
 #pragma unroll
@@ -88,6 +99,25 @@ __device__ __forceinline__ int ap_find_tile(const ApArgs& a, int t, int4& u) {
     t -= __shfl_sync(0xffffffffu, end, 31);
   }
   return -1;
+}
+// Whether the tiles of row m's query rows are among the tiles_p that the grid has. They are, unless
+// units overlap: those of disjoint units are at most tiles_p. Whole warps call.
+__device__ __forceinline__ bool ap_row_has_tile(const ApArgs& a, int m) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int u0 = 0; u0 < a.num_units; u0 += 32) {
+    int tiles = 0, own = -1;
+    if (u0 + lane < a.num_units) {
+      const int4 v = a.units[u0 + lane];
+      tiles = ap_unit_tiles(a, v);
+      if (tiles > 0 && m >= v.x && m - v.x < v.y) own = ((m - v.x) * a.G + a.G - 1) >> a.tr_sh;
+    }
+    const uint32_t hit = __ballot_sync(0xffffffffu, own >= 0);
+    const int l = hit != 0u ? __ffs(hit) - 1 : 32;
+    before += __reduce_add_sync(0xffffffffu, lane < l ? tiles : 0);
+    if (hit != 0u) return before + __shfl_sync(0xffffffffu, own, l) < a.tiles_p;
+  }
+  return true;  // in no unit
 }
 // The row's cache slot and own length, or false when either lies outside the cache.
 __device__ __forceinline__ bool ap_row(const ApArgs& a, int m, int& slot, int& len) {

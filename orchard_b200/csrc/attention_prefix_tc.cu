@@ -90,10 +90,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   int4 u;
   const int i0 = ap_find_tile(a, tile, u);
   if (i0 < 0) return;
-  if (!ap_unit_ok(a, u)) {
-    if (tid == 0) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
-    return;
-  }
   const int n = min(C::Rows, u.y * a.G - i0);
   const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
   if (j0 >= j1) return;
