@@ -67,12 +67,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint8_t* sV = sm + C::OffV;
   uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + C::Bytes);
   uint64_t* vfull = kfull + 2;
-  uint64_t* sready = vfull + 2;  // scores written: also, the K slot is free
+  uint64_t* sready = vfull + 2;  // scores written: also (not PAIR) the K slot is free
   uint64_t* sread = sready + 2;  // scores read
   uint64_t* pready = sread + 2;   // [group][half]: weights of the block's first and last 64 keys
   uint64_t* pvdone = pready + 4;  // four, block i's at i & 3: weights used, the V slot is free
   uint64_t* refset = pvdone + 4;  // [group][warp of the group]: the rows' ref after its block
-  uint64_t* qfull = refset + 8;
+  uint64_t* kfree = refset + 8;   // [slot], PAIR: the last group's product has read the slot
+  uint64_t* vfree = kfree + 2;
+  uint64_t* qfull = vfree + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -104,6 +106,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&sread[i], 4);  // one lane per warp of the group
       mbar_init(&pready[2 * i], 4);
       mbar_init(&pready[2 * i + 1], 4);
+      mbar_init(&kfree[i], 1);
+      mbar_init(&vfree[i], 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&pvdone[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&refset[i], 1);
@@ -129,18 +133,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         mbar_expect_tx(bar, (uint32_t)C::Tile);
         for (int d = 0; d < HD / 64; ++d) tma_load_2d(to + (i & 1) * C::Tile + d * C::Atom, map, bar, d * 64, y0 + i * kApTcKeys);
       };
-      // a slot is free after the products of two blocks before; in the order in which they end
+      // A slot is free after the products of two blocks before; in the order in which they end. The
+      // barriers waited for pass once for each use of a slot, so none can be two phases ahead (a
+      // parity would name the wrong one): the next use is this thread's own.
       auto load_k = [&](int i) {
-        uint64_t* bar = PAIR ? &sready[groups - 1] : &sready[i & 1];
-        const int phase = PAIR ? i - 2 : (i >> 1) - 1;
-        if (i >= 2 && !mbar_wait_f(bar, (uint32_t)phase & 1, failed)) return false;
+        uint64_t* bar = PAIR ? &kfree[i & 1] : &sready[i & 1];
+        if (i >= 2 && !mbar_wait_f(bar, (uint32_t)((i >> 1) - 1) & 1, failed)) return false;
         load(sK, &tmk, &kfull[i & 1], i);
         ik = i + 1;
         return true;
       };
       auto load_v = [&](int i) {
-        uint64_t* bar = PAIR ? &pvdone[groups - 1] : &pvdone[(i - 2) & 3];
-        const int phase = PAIR ? i - 2 : (i - 2) >> 2;
+        uint64_t* bar = PAIR ? &vfree[i & 1] : &pvdone[(i - 2) & 3];
+        const int phase = PAIR ? (i >> 1) - 1 : (i - 2) >> 2;
         if (i >= 2 && !mbar_wait_f(bar, (uint32_t)phase & 1, failed)) return false;
         load(sV, &tmv, &vfull[i & 1], i);
         iv = i + 1;
@@ -177,6 +182,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         umma_f16_ss_warp(tmem + g * 128, sw128_desc(smem_u32(q + (kk >> 2) * C::Atom)) + 2 * (kk & 3),
                          sw128_desc(smem_u32(sK + (i & 1) * C::Tile + (kk >> 2) * C::Atom)) + 2 * (kk & 3), kIdescS, kk > 0);
       umma_commit_warp(&sready[g]);
+      if (PAIR && g == groups - 1 && i + 2 < nb) umma_commit_warp(&kfree[i & 1]);
       ++issued_s[g];
     };
     // accumulator of g += weights of block i . V, as the two halves of the weights come
@@ -196,6 +202,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
       }
       umma_commit_warp(&pvdone[done]);
+      if (PAIR && g == groups - 1 && i + 2 < nb) umma_commit_warp(&vfree[i & 1]);
       ++issued_o[done];
       return true;
     };
