@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* refset = pvdone + 4;  // [group][warp of the group]: the rows' ref after its block
   uint64_t* kfree = refset + 8;   // [slot], PAIR: the last group's product has read the slot
   uint64_t* vfree = kfree + 2;
-  uint64_t* qfull = vfree + 2;
+  uint64_t* drain = vfree + 2;  // every product issued has ended
+  uint64_t* qfull = drain + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
   volatile int* failed = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -111,6 +112,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     for (int i = 0; i < 4; ++i) mbar_init(&pvdone[i], 1);
     for (int i = 0; i < 8; ++i) mbar_init(&refset[i], 1);
+    mbar_init(drain, 1);
     mbar_init(qfull, 8);  // one lane per warp of the groups
     *failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -158,16 +160,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         else
           ok = (i + 1 >= nb || load_k(i + 1)) && load_v(i);
       }
-      if (!ok) {  // loads still in flight when the others gave up
-        *failed = 1;
-        for (int i = max(0, ik - 2); i < ik; ++i) mbar_wait(&kfull[i & 1], (uint32_t)(i >> 1) & 1);
-        for (int i = max(0, iv - 2); i < iv; ++i) mbar_wait(&vfull[i & 1], (uint32_t)(i >> 1) & 1);
-      }
+      if (!ok) *failed = 1;
+      // whoever gave up, no load may still be in flight when the CTA ends
+      for (int i = max(0, ik - 2); i < ik; ++i) mbar_wait(&kfull[i & 1], (uint32_t)(i >> 1) & 1);
+      for (int i = max(0, iv - 2); i < iv; ++i) mbar_wait(&vfull[i & 1], (uint32_t)(i >> 1) & 1);
     }
     __syncwarp();
   } else if (warp == 9) {
     // every lane waits and computes the descriptors, an elected one issues
-    int issued_s[2] = {0, 0}, issued_o[4] = {0, 0, 0, 0};
     auto wait = [&](uint64_t* bar, int phase) {
       return __all_sync(0xffffffffu, mbar_wait_f(bar, (uint32_t)phase & 1, failed)) != 0;
     };
@@ -183,7 +183,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                          sw128_desc(smem_u32(sK + (i & 1) * C::Tile + (kk >> 2) * C::Atom)) + 2 * (kk & 3), kIdescS, kk > 0);
       umma_commit_warp(&sready[g]);
       if (PAIR && g == groups - 1 && i + 2 < nb) umma_commit_warp(&kfree[i & 1]);
-      ++issued_s[g];
     };
     // accumulator of g += weights of block i . V, as the two halves of the weights come
     auto weigh = [&](int g, int i, int done) {
@@ -203,7 +202,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       umma_commit_warp(&pvdone[done]);
       if (PAIR && g == groups - 1 && i + 2 < nb) umma_commit_warp(&vfree[i & 1]);
-      ++issued_o[done];
       return true;
     };
     bool ok = arrived(kfull, 0) && wait(qfull, 0);
@@ -234,13 +232,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         ok = ok && weigh(w, i, i & 3) && arrived(vfull, i + 1);
       }
     }
-    if (!ok) {  // products still running
-      *failed = 1;
-      for (int w = 0; w < 2; ++w)
-        if (issued_s[w]) mbar_wait(&sready[w], (uint32_t)(issued_s[w] - 1) & 1);
-      for (int w = 0; w < 4; ++w)
-        if (issued_o[w]) mbar_wait(&pvdone[w], (uint32_t)(issued_o[w] - 1) & 1);
-    }
+    if (!ok) *failed = 1;
+    // Whoever gave up, no product may still be running when tensor memory is freed; some may have no
+    // commit of their own (a block's first half, when its second half's weights did not come).
+    umma_commit_warp(drain);
+    mbar_wait(drain, 0);
     __syncwarp();
   } else {
     if (tid < n) reinterpret_cast<int*>(sm + C::OffRec)[tid] = (u.x + (i0 + tid) / a.G) * a.nh + kv * a.G + (i0 + tid) % a.G;

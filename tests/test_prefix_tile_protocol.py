@@ -211,3 +211,45 @@ def test_the_model_sees_a_barrier_that_passes_every_block():
             assert "producer" in str(e)
             late += 1
     assert late > 0
+
+
+@pytest.mark.parametrize("groups", [1, 2])
+def test_nothing_runs_on_after_the_issuer_has_left(groups):
+    """The issuer gives up at any of its waits, for whatever reason: its last commit comes after every
+    product, those of a half block among them, and it leaves when that has passed."""
+    for stop in range(40):
+        m, drain = Model(random.Random(stop)), Barrier("drain")
+        m.put = lambda *a: None  # what the products read no longer matters
+        roles = pair(m, 6, groups, False)
+
+        def issuer(role=roles["issuer"], stop=stop):
+            for n, w in enumerate(role):
+                if n == stop:
+                    break
+                w[0].phase = w[1] + 1  # as if it had come
+                yield pause_at()
+            m.commit(drain)
+            yield (drain, 0)
+            assert not m.products
+            done.append(stop)
+
+        done = []
+        m.mem = _Anything()
+        m.run({"issuer": issuer()})
+        assert done == [stop]
+
+
+def pause_at():
+    b = Barrier("pause")
+    b.arrive()
+    return (b, 0)
+
+
+class _Anything(dict):
+    def get(self, place, default=None):
+        return _Any()
+
+
+class _Any:
+    def __eq__(self, other):
+        return True
