@@ -304,7 +304,8 @@ int orch_embed_rows(const int32_t* ids, const void* table, int table_dt, float* 
  * [prefix_cap][head_dim]; `units` (device, 16-byte aligned) lists num_units records of four
  * int32 (row0, rows, prefix, length): rows row0 .. row0 + rows - 1 (1..128 of them) attend to
  * the first `length` (<= max_prefix <= prefix_cap) entries of prefix `prefix`. A row belongs to
- * one unit at most (num_units <= M); one in none has no prefix. Row m also attends to the first lens[m]
+ * one unit at most (num_units <= M); one in none has no prefix (with max_prefix 0, prefix_k,
+ * prefix_v and `units` may be NULL). Row m also attends to the first lens[m]
  * (<= max_own <= max_seq) entries of slot slots[m] (NULL = m) of the caches, laid out
  * [num_slots][num_kv_heads][max_seq][head_dim]; entries past that are not read. Query and
  * entries carry their rotations, so the order of the entries does not matter. A row with

@@ -594,7 +594,7 @@ __device__ __forceinline__ bool ap_row_prefix(const ApArgs& a, int m, int& pslot
   pslot = (int)__reduce_add_sync(0xffffffffu, (unsigned)z);  // one lane's at most, when in <= 1
   plen = (int)__reduce_add_sync(0xffffffffu, (unsigned)w);
   if (__any_sync(0xffffffffu, bad) || in > 1) return false;
-  if (TILES && (__reduce_add_sync(0xffffffffu, (unsigned)tiles) > (unsigned)a.tiles_p || __any_sync(0xffffffffu, tiles == kMany)) &&
+  if (TILES && plen > 0 && (__reduce_add_sync(0xffffffffu, (unsigned)tiles) > (unsigned)a.tiles_p || __any_sync(0xffffffffu, tiles == kMany)) &&
       !ap_row_has_tile(a, m)) {
     if (lane == 0) atomicOr(a.check, 2u);
     return false;
@@ -893,8 +893,8 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.row = (size_t)M * nkv <= kApDirectPairs && (some ? max_prefix : 0) + (uint64_t)max_own <= kApDirectKeys &&
              (!track || (M == 1 && p.tiles_o == 1));
   if (p.row) p.tc = 0;
-  // one range per row in all: nothing to join either
-  p.direct = p.row || (!some && p.S_o == 1 && !track);
+  // one range per row in all, and no unit that could reject a row: nothing to join either
+  p.direct = p.row || (num_units == 0 && p.S_o == 1 && !track);
   const size_t mh = (size_t)M * nh, S = p.S_p + p.S_o;
   p.acc_floats = p.direct ? 0 : mh * S * hd;
   p.stat_floats = p.direct ? 0 : (mh * S * 2 + 3) / 4 * 4;
@@ -1015,7 +1015,7 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.kp = static_cast<const __half*>(prefix_k);
   a.vp = static_cast<const __half*>(prefix_v);
   a.units = reinterpret_cast<const int4*>(units);
-  a.num_units = p.S_p ? (int)num_units : 0;
+  a.num_units = units ? (int)num_units : 0;  // with max_prefix 0 they may be left out
   a.max_prefix = (int)max_prefix;
   a.prefix_cap = (int)prefix_cap;
   a.num_prefix = (int)num_prefix;

@@ -56,10 +56,14 @@ __host__ __device__ __forceinline__ int ap_range(int n, int S, int block = kApKe
   return (per + block - 1) / block * block;
 }
 
-// A unit that names rows, a prefix slot and a length inside what the call was given.
+// A unit's prefix is one of the call's; with max_prefix 0 there are none, and its number does not matter.
+__device__ __forceinline__ bool ap_unit_prefix_ok(const ApArgs& a, const int4& u) {
+  return a.max_prefix == 0 || (u.z >= 0 && u.z < a.num_prefix);
+}
+// A unit that names rows, a prefix and a length inside what the call was given.
 __device__ __forceinline__ bool ap_unit_ok(const ApArgs& a, const int4& u) {
   return u.y >= 1 && u.y <= kApMaxUnitRows && u.x >= 0 && u.x < a.M && u.y <= a.M - u.x && u.w >= 0 &&
-         u.w <= a.max_prefix && u.z >= 0 && u.z < a.num_prefix;
+         u.w <= a.max_prefix && ap_unit_prefix_ok(a, u);
 }
 // Row tiles of a unit; a rejected one has none.
 __device__ __forceinline__ int ap_unit_tiles(const ApArgs& a, const int4& u) {
@@ -69,7 +73,7 @@ __device__ __forceinline__ int ap_unit_tiles(const ApArgs& a, const int4& u) {
 __device__ __forceinline__ void ap_report_units(const ApArgs& a) {
   for (int i = threadIdx.x; i < a.num_units; i += blockDim.x) {
     const int4 u = a.units[i];
-    if (!ap_unit_ok(a, u)) atomicOr(a.check, u.z < 0 || u.z >= a.num_prefix ? 8u : 2u);
+    if (!ap_unit_ok(a, u)) atomicOr(a.check, ap_unit_prefix_ok(a, u) ? 2u : 8u);
   }
 }
 // Row tile t of all units, in their order: its unit (in u) and its first query row, or -1 past

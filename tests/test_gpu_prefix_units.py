@@ -88,3 +88,22 @@ def test_units_that_overlap(rows, units, hd, nh, nkv, bound):
             assert not mass[t].any(), m
         else:
             assert m >= last[0] and close(got[m], want[m], limit[m]) and close(mass[t], wmass[t], mlimit[t]), m
+
+
+@pytest.mark.parametrize("track", [False, True])
+@pytest.mark.parametrize("rows,cap", [(3, 10), (3, 700), (70, 30)])
+def test_units_without_room_for_a_prefix(rows, cap, track):
+    """max_prefix 0: units of length 0 are as none; a longer one is out of range, its rows are left
+    unwritten and reported."""
+    lens = [(7 * i) % cap for i in range(rows)]
+    host = case(rows, 64, 4, 2, [], lens, cap, pcap=1)
+    want, limit, wmass, mlimit = expected(host, [])
+    for units, left in (([(0, 2, 0, 0), (2, 1, 0, 0)], None), ([(0, 1, 0, 0), (1, 1, 0, 5)], 1)):
+        mass = torch.zeros((rows, 2, cap), device="cuda") if track else None
+        got = go(host, units, 0, mass)
+        assert flags() == (0 if left is None else 2)
+        keep = [r for r in range(rows) if r != left]
+        assert close(got[keep], want[keep], limit[keep]) and (left is None or bool((got[left] == 7).all()))
+        if track:
+            at, mass = host[7][keep], mass.cpu().numpy()
+            assert close(mass[at], wmass[at], mlimit[at]) and (left is None or not mass[host[7][left]].any())
