@@ -13,11 +13,11 @@
 // that K/V head), so the prefix is read once for all of them; another CTA takes a range of
 // one row's own entries for its G heads. Both run the same tensor-core tile: S = Q K^T in
 // m16n8k16 MMAs (exact products of fp16 values, fp32 sums), an online softmax in fp32, O += P V
-// with P rounded to fp16. That rounding costs up to 2^-11 of each weight, as much as the rounding
-// of the fp16 output; the sums l take the unrounded weights, and P is scaled by 2^10 so that
-// weights down to 2^-24 of the largest stay normal numbers. With few rows (`fine`), where the
-// products are not what takes the time, P V adds what the rounding left off as a second product
-// (64 rows behind 4,096 entries: 65.6 us without, 70.4 with; one row of 577: 9.0 and 9.2).
+// with P in two fp16 terms, as in the prefill kernel: hi = fp16(p), lo = fp16(p - hi), a product
+// each. One term alone would be off by up to 2^-11 of each weight, as much as the rounding of the
+// fp16 output (64 x 32 heads behind 4,096 entries: 72.4 us a call, 71.8 with one term; 32 x 8 heads
+// x 4, tracked: 41.7 and 39.6). The sums l take the fp32 weights, and P is scaled by 2^10 so that
+// weights down to 2^-24 of the largest are normal numbers.
 //
 // Layout of a CTA: 4 warps. A tile of 64 rows gives each warp 16 rows and all 64 keys of a
 // block; a tile of 16 or 32 rows splits the block's keys over 4 or 2 warps instead, whose
@@ -69,7 +69,7 @@ struct ApKeys {
 
 // One tile: query rows i0 .. i0 + n - 1 of the (row, head of kv) pairs starting at row m0, over
 // `keys`; partials go to range `split`. The statistics of the rows stay in shared memory.
-template <int HD, int WR, bool FINE>
+template <int HD, int WR>
 __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, int kv, const ApKeys& keys, int split) {
   constexpr int WK = 4 / WR, TR = 16 * WR, TILE = kApKeys * HD, KT = kApKeys / 8 / WK;
   extern __shared__ __align__(16) uint8_t ap_smem[];
@@ -215,16 +215,14 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
     }
 #pragma unroll
     for (int j = 0; j < KT / 2; ++j) {
-      uint32_t hi[4], lo[4] = {0u, 0u, 0u, 0u};
+      uint32_t hi[4], lo[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const float p0 = sc[2 * j + (x >> 1)][2 * (x & 1)], p1 = sc[2 * j + (x >> 1)][2 * (x & 1) + 1];
         const __half2 h = __floats2half2_rn(p0, p1);
+        const float2 f = __half22float2(h);
         hi[x] = h2_bits(h);
-        if (FINE) {
-          const float2 f = __half22float2(h);
-          lo[x] = h2_bits(__floats2half2_rn(p0 - f.x, p1 - f.y));
-        }
+        lo[x] = h2_bits(__floats2half2_rn(p0 - f.x, p1 - f.y));
       }
 #pragma unroll
       for (int d = 0; d < HD / 8; d += 2) {
@@ -232,10 +230,8 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
         ap_ldsm4_t(vs + ap_at<HD>(8 * kt0 + 16 * j + 8 * (lm & 1) + lr, d + (lm >> 1)), bb);
         mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], bb[0], bb[1]);
         mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], bb[2], bb[3]);
-        if (FINE) {
-          mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
-          mma_16816(o[d + 1], lo[0], lo[1], lo[2], lo[3], bb[2], bb[3]);
-        }
+        mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
+        mma_16816(o[d + 1], lo[0], lo[1], lo[2], lo[3], bb[2], bb[3]);
       }
     }
     __syncthreads();  // buffer b & 1 is free for block b + 2
@@ -320,7 +316,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 // [j0, j1), 16 keys at a time through the warp's own ring of two stages. Where there are enough
 // rows and heads, four of these per CTA need no barrier and no join across warps, and a quarter of
 // the CTAs: AAA.
-template <int HD, bool FINE>
+template <int HD>
 __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __half* k, const __half* v, int j0, int j1,
                                         int split, float* srow) {
   constexpr int KEYS = 16, TILE = KEYS * HD, CPR = HD / 8, RS = 32 / CPR;  // 16-byte pieces per row, rows per pass
@@ -409,7 +405,7 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
     const float al0 = ap_exp2(m0 - (mn0 == -INFINITY ? 0.f : mn0)), al1 = ap_exp2(m1 - (mn1 == -INFINITY ? 0.f : mn1));
     m0 = mn0;
     m1 = mn1;
-    uint32_t hi[4], lo[4] = {0u, 0u, 0u, 0u};
+    uint32_t hi[4], lo[4];
     float rs0 = 0.f, rs1 = 0.f;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
@@ -420,11 +416,9 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
       else
         rs0 += p0 + p1;
       const __half2 h = __floats2half2_rn(p0, p1);
+      const float2 w = __half22float2(h);
       hi[x] = h2_bits(h);
-      if (FINE) {
-        const float2 w = __half22float2(h);
-        lo[x] = h2_bits(__floats2half2_rn(p0 - w.x, p1 - w.y));
-      }
+      lo[x] = h2_bits(__floats2half2_rn(p0 - w.x, p1 - w.y));
     }
     l0 = l0 * al0 + rs0;
     l1 = l1 * al1 + rs1;
@@ -443,10 +437,8 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
       ap_ldsm4_t(vs + ap_at<HD>(8 * (lm & 1) + lr, d + (lm >> 1)), bb);
       mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], bb[0], bb[1]);
       mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], bb[2], bb[3]);
-      if (FINE) {
-        mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
-        mma_16816(o[d + 1], lo[0], lo[1], lo[2], lo[3], bb[2], bb[3]);
-      }
+      mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
+      mma_16816(o[d + 1], lo[0], lo[1], lo[2], lo[3], bb[2], bb[3]);
     }
     __syncwarp();  // stage b & 1 is free for block b + 2
   }
@@ -478,8 +470,7 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
 
 // WRP, WRO: warps along the rows of a prefix tile and of an own tile (WRP 0: no prefix here; WRO 0:
 // own entries by single warps).
-// FINE: weights in two fp16 terms.
-template <int HD, int WRP, int WRO, bool FINE>
+template <int HD, int WRP, int WRO>
 __device__ __forceinline__ void ap_work(const ApArgs& a) {
   int b = blockIdx.x;
   if (a.num_units > 0) {  // the first CTA reports the rejected units
@@ -501,7 +492,7 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
     const int per = ap_range(u.w, a.S_p, a.blk_p), j0 = split * per, j1 = min(u.w, j0 + per);
     if (j0 >= j1) return;
     const size_t base = ((size_t)u.z * a.nkv + kv) * a.prefix_cap * HD;
-    ap_tile<HD, WRP ? WRP : 1, FINE>(a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
+    ap_tile<HD, WRP ? WRP : 1>(a, u.x, i0, n, kv, ApKeys{a.kp + base, a.vp + base, j0, j1, nullptr, nullptr, 0, nullptr, false},
                    split);
     return;
   }
@@ -526,7 +517,7 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
       return;
     }
     const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
-    ap_warp<HD, FINE>(a, m, kv, a.kc + base, a.vc + base, j0, j1, a.S_p + split,
+    ap_warp<HD>(a, m, kv, a.kc + base, a.vc + base, j0, j1, a.S_p + split,
                       a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr);
     return;
   }
@@ -552,18 +543,18 @@ __device__ __forceinline__ void ap_work(const ApArgs& a) {
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD;
   float* srow = a.mass ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile<HD, WR, FINE>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
+  ap_tile<HD, WR>(a, m, i0, n, kv, ApKeys{a.kc + base, a.vc + base, j0, j1, nullptr, nullptr, 0, srow, false},
                  a.S_p + split);
 }
 
-template <int HD, int WRP, int WRO, bool FINE>
+template <int HD, int WRP, int WRO>
 __global__ void __launch_bounds__(128, 3) attn_prefix_kernel(const ApArgs a) {
   pdl_trigger();
   // Beside the prefix's own kernel, launched just before: that kernel waited for everything
   // earlier before it let this one start, and the two share no output, so they run together.
   // The first CTA stays until it has ended, so that whoever waits for this grid waits for both.
   if (!a.tc) pdl_wait();
-  ap_work<HD, WRP, WRO, FINE>(a);
+  ap_work<HD, WRP, WRO>(a);
   if (a.tc && blockIdx.x == 0) pdl_wait();
 }
 
@@ -634,7 +625,7 @@ __global__ void __launch_bounds__(128, 3) attn_prefix_row_kernel(const ApArgs a)
   }
   const size_t base = ((size_t)slot * a.nkv + kv) * a.max_seq * HD, pb = ((size_t)pslot * a.nkv + kv) * a.prefix_cap * HD;
   float* srow = a.mass && len > 0 ? a.scores + ((size_t)m * a.nh + kv * a.G) * a.lds : nullptr;
-  ap_tile<HD, WRO, true>(a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
+  ap_tile<HD, WRO>(a, m, i0, n, kv, ApKeys{a.kp + pb, a.vp + pb, 0, plen, a.kc + base, a.vc + base, len, srow, true}, 0);
 }
 
 template <int V>
@@ -903,7 +894,7 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   return p;
 }
 
-template <int HD, int WRP, int WRO, bool FINE>
+template <int HD, int WRP, int WRO>
 int ap_launch_shape(ApArgs a, cudaStream_t st) {
   constexpr int kSmem = 4 * kApKeys * HD * 2;
   constexpr int kJoin = 64 * (HD + 4) * 4 + 64 * 8;  // WK x TR = 64 rows of O and their statistics
@@ -911,7 +902,7 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
   static bool attr_done[64] = {};
   const int dev = device_index();
   if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD, WRP, WRO, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<HD, WRP, WRO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     ORCH_CUDA(cudaFuncSetAttribute(attn_prefix_row_kernel<HD, WRO ? WRO : 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr_done[dev] = true;
   }
@@ -928,7 +919,7 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
   }
   const size_t own = (size_t)a.M * a.nkv * a.S_o * a.tiles_o, blocks = (size_t)a.blocks_p + (WRO ? own : (own + 3) / 4) + (a.num_units > 0);
   if (blocks > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads for one launch");
-  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO, FINE>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
+  ORCH_CUDA(launch_k_pdl(a.tc != 0, attn_prefix_kernel<HD, WRP, WRO>, dim3((unsigned)blocks), dim3(128), smem, st, none, a));
   if (a.direct) return check_launch("attention_prefix");
   const int blocks_out = (int)(((size_t)a.M * a.nh + 3) / 4);
   const int chunks = a.mass ? (a.max_own + kMassEntries - 1) / kMassEntries : 0;
@@ -939,11 +930,6 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
   return check_launch("attention_prefix");
 }
 
-template <int HD, int WRP, int WRO>
-int ap_launch_wr(const ApArgs& a, cudaStream_t st) {
-  return a.fine ? ap_launch_shape<HD, WRP, WRO, true>(a, st) : ap_launch_shape<HD, WRP, WRO, false>(a, st);
-}
-
 // A tile of a unit has at least the rows of a tile of one row, so wr_p >= wr_o; with head_dim 64
 // or 128 it has 64 rows only where a row's heads already fill that.
 template <int HD>
@@ -951,17 +937,17 @@ int ap_launch(const ApArgs& a, cudaStream_t st) {
   const int p = a.tc || a.row || a.blocks_p == 0 ? 0 : a.wr_p;
   const int o = a.by_warp ? 0 : a.wr_o;
   if (p == 0)
-    return o == 0 ? ap_launch_wr<HD, 0, 0>(a, st) : o == 1 ? ap_launch_wr<HD, 0, 1>(a, st)
-         : o == 2 ? ap_launch_wr<HD, 0, 2>(a, st) : ap_launch_wr<HD, 0, 4>(a, st);
-  if (p == 1) return o == 0 ? ap_launch_wr<HD, 1, 0>(a, st) : ap_launch_wr<HD, 1, 1>(a, st);
+    return o == 0 ? ap_launch_shape<HD, 0, 0>(a, st) : o == 1 ? ap_launch_shape<HD, 0, 1>(a, st)
+         : o == 2 ? ap_launch_shape<HD, 0, 2>(a, st) : ap_launch_shape<HD, 0, 4>(a, st);
+  if (p == 1) return o == 0 ? ap_launch_shape<HD, 1, 0>(a, st) : ap_launch_shape<HD, 1, 1>(a, st);
   if (p == 2)
-    return o == 0 ? ap_launch_wr<HD, 2, 0>(a, st) : o == 1 ? ap_launch_wr<HD, 2, 1>(a, st) : ap_launch_wr<HD, 2, 2>(a, st);
+    return o == 0 ? ap_launch_shape<HD, 2, 0>(a, st) : o == 1 ? ap_launch_shape<HD, 2, 1>(a, st) : ap_launch_shape<HD, 2, 2>(a, st);
   if constexpr (HD == 32) {
-    if (o == 0) return ap_launch_wr<HD, 4, 0>(a, st);
-    if (o == 1) return ap_launch_wr<HD, 4, 1>(a, st);
-    if (o == 2) return ap_launch_wr<HD, 4, 2>(a, st);
+    if (o == 0) return ap_launch_shape<HD, 4, 0>(a, st);
+    if (o == 1) return ap_launch_shape<HD, 4, 1>(a, st);
+    if (o == 2) return ap_launch_shape<HD, 4, 2>(a, st);
   }
-  return ap_launch_wr<HD, 4, 4>(a, st);
+  return ap_launch_shape<HD, 4, 4>(a, st);
 }
 
 bool ap_shape_ok(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd) {
@@ -1051,7 +1037,6 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.direct = p.direct;
   a.row = p.row;
   a.by_warp = p.by_warp;
-  a.fine = (uint64_t)M * num_kv_heads <= kApDirectPairs;
   a.acc = static_cast<float*>(workspace);
   a.stat = reinterpret_cast<float2*>(a.acc + p.acc_floats);
   a.scores = a.acc + p.acc_floats + p.stat_floats;

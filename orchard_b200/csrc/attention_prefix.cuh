@@ -35,7 +35,6 @@ struct ApArgs {
   int blocks_p;          // CTAs of the prefix part
   int row;               // few rows and keys: a CTA per row and K/V head takes all of them
   int by_warp;           // own entries by single warps, four rows and K/V heads per CTA
-  int fine;              // weights in two fp16 terms
   int direct;            // the output is written by the attention kernel: nothing to join
   float* acc;            // [M * nh][S][HD]
   float2* stat;          // [M * nh][S]: (max, sum), in powers of two

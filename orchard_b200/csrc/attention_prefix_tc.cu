@@ -15,18 +15,21 @@
 //  * one warp issues the products, a lane elected at each;
 //  * a thread of a group owns one query row and holds a block's 128 scores in registers: maximum,
 //    weights and sum need no shuffles. A row's weights are scaled by `ref`, which moves only when
-//    a maximum exceeds it by more than 2^7 (held weights then reach 2^15 at most, and stay
-//    normal down to 2^-22 of the largest; any scale gives the same quotient); then the
-//    accumulator is rescaled before the block's product.
-// Alternate blocks share one accumulator, so that weights need not lie over scores and the scores
-// of block i + 2 are under way as soon as block i's have been read; `ref` passes from block to
-// block through shared memory right after each maximum. With PAIR each group has its own
-// accumulator and the weights lie over the scores they came from.
+//    a maximum exceeds it by more than 2^7 (held weights then reach 2^15 at most; any scale
+//    gives the same quotient); then the accumulator is rescaled before the block's product.
+//    Each weight is held in two fp16 terms, hi = fp16(p) and lo = fp16(p - hi), 22 bits together:
+//    one alone would be off by up to 2^-11 of the weight, as much as the output's own rounding.
+// The weights of a block lie over the scores they came from, whose 128 columns their two terms
+// fill. Alternate blocks share one accumulator and take three score buffers in turn: the scores of
+// block i + 2 go where block i - 1's weights were, under way while block i's become weights;
+// `ref` passes from block to block through shared memory right after each maximum. With PAIR each
+// group has its own accumulator and one buffer.
 // The CTA writes one record per row for the join. Keys past the range are masked, their V rows
 // zeroed in shared memory (whatever lies there in the prefix region could be a NaN).
 //
-// Tensor memory (512 columns): scores at 0 and 128; weights (fp16) at 256 and 320 and the
-// accumulator at 384, or (PAIR) accumulators at 256 and 256 + HD. Every mbarrier wait is bounded;
+// Tensor memory (512 columns): score buffers at 0, 128 and 256 and the accumulator at 384, or
+// (PAIR) at 0 and 128, accumulators at 256 and 256 + HD. Each 32 keys of a buffer's weights have
+// the 16 columns of their hi terms, then the 16 of their lo terms. Every mbarrier wait is bounded;
 // one that runs out sets device check bit 256.
 #include "attention_prefix.cuh"
 #include "tcgen05.cuh"
@@ -50,8 +53,8 @@ struct PtCfg {
   static constexpr int OffRef = Bytes + 256;  // a row's ref (floats), behind the barriers
   static constexpr int OffRec = OffRef + kApTcRows * 4;  // a row's number among all (row, head) pairs
   static constexpr int Smem = OffRec + Rows * 4;
-  static constexpr uint32_t ColP = PAIR ? 0 : 256, StepP = PAIR ? 128 : 64;    // weights of group g
-  static constexpr uint32_t ColO = PAIR ? 256 : 384, StepO = PAIR ? HD : 0;  // its accumulator
+  static constexpr int Bufs = PAIR ? 2 : 3;                                  // score buffers of 128 columns
+  static constexpr uint32_t ColO = PAIR ? 256 : 384, StepO = PAIR ? HD : 0;  // accumulator of group g
 };
 
 __device__ __forceinline__ void pt_groups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -67,11 +70,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint8_t* sV = sm + C::OffV;
   uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + C::Bytes);
   uint64_t* vfull = kfull + 2;
-  uint64_t* sready = vfull + 2;  // scores written: also (not PAIR) the K slot is free
-  uint64_t* sread = sready + 2;  // scores read
-  uint64_t* pready = sread + 2;   // [group][half]: weights of the block's first and last 64 keys
-  uint64_t* pvdone = pready + 4;  // four, block i's at i & 3: weights used, the V slot is free
-  uint64_t* refset = pvdone + 4;  // [group][warp of the group]: the rows' ref after its block
+  // Of a score buffer; a buffer's phases are its blocks. (Barriers by the block's parity would not
+  // do: three blocks are under way, and a parity names one of two phases.)
+  uint64_t* sready = vfull + 2;   // scores written: also (not PAIR) the K slot is free
+  uint64_t* pready = sready + 3;  // [buffer][half]: weights of the block's first and last 64 keys
+  uint64_t* pvdone = pready + 6;  // weights used: also (not PAIR) the V slot is free
+  uint64_t* refset = pvdone + 3;  // [group][warp of the group]: the rows' ref after its block
   uint64_t* kfree = refset + 8;   // [slot], PAIR: the last group's product has read the slot
   uint64_t* vfree = kfree + 2;
   uint64_t* drain = vfree + 2;  // every product issued has ended
@@ -103,14 +107,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&kfull[i], 1);
       mbar_init(&vfull[i], 1);
-      mbar_init(&sready[i], 1);
-      mbar_init(&sread[i], 4);  // one lane per warp of the group
-      mbar_init(&pready[2 * i], 4);
-      mbar_init(&pready[2 * i + 1], 4);
       mbar_init(&kfree[i], 1);
       mbar_init(&vfree[i], 1);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&pvdone[i], 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&sready[i], 1);
+      mbar_init(&pready[2 * i], 4);  // one lane per warp of the group
+      mbar_init(&pready[2 * i + 1], 4);
+      mbar_init(&pvdone[i], 1);
+    }
     for (int i = 0; i < 8; ++i) mbar_init(&refset[i], 1);
     mbar_init(drain, 1);
     mbar_init(qfull, 8);  // one lane per warp of the groups
@@ -139,15 +144,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // barriers waited for pass once for each use of a slot, so none can be two phases ahead (a
       // parity would name the wrong one): the next use is this thread's own.
       auto load_k = [&](int i) {
-        uint64_t* bar = PAIR ? &kfree[i & 1] : &sready[i & 1];
-        if (i >= 2 && !mbar_wait_f(bar, (uint32_t)((i >> 1) - 1) & 1, failed)) return false;
+        uint64_t* bar = PAIR ? &kfree[i & 1] : &sready[(i - 2) % 3];
+        const int phase = PAIR ? (i >> 1) - 1 : (i - 2) / 3;
+        if (i >= 2 && !mbar_wait_f(bar, (uint32_t)phase & 1, failed)) return false;
         load(sK, &tmk, &kfull[i & 1], i);
         ik = i + 1;
         return true;
       };
       auto load_v = [&](int i) {
-        uint64_t* bar = PAIR ? &vfree[i & 1] : &pvdone[(i - 2) & 3];
-        const int phase = PAIR ? (i >> 1) - 1 : (i - 2) >> 2;
+        uint64_t* bar = PAIR ? &vfree[i & 1] : &pvdone[(i - 2) % 3];
+        const int phase = PAIR ? (i >> 1) - 1 : (i - 2) / 3;
         if (i >= 2 && !mbar_wait_f(bar, (uint32_t)phase & 1, failed)) return false;
         load(sV, &tmv, &vfull[i & 1], i);
         iv = i + 1;
@@ -173,35 +179,41 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     };
     // The waits for K and V (`arrived`) are placed where products are running, not before them.
     auto arrived = [&](uint64_t* full, int i) { return i >= nb || wait(&full[i & 1], i >> 1); };
-    // block i's scores into buffer g, from rows 128 g of the tile (PAIR) or all of them
-    auto scores = [&](int g, int i) {
+    // block i's scores into buffer b, from rows 128 g of the tile (PAIR: g is b) or all of them
+    auto scores = [&](int b, int i) {
       tc_fence_after();
-      uint8_t* q = sm + (PAIR ? g * C::Tile : 0);
+      uint8_t* q = sm + (PAIR ? b * C::Tile : 0);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk)
-        umma_f16_ss_warp(tmem + g * 128, sw128_desc(smem_u32(q + (kk >> 2) * C::Atom)) + 2 * (kk & 3),
+        umma_f16_ss_warp(tmem + b * 128, sw128_desc(smem_u32(q + (kk >> 2) * C::Atom)) + 2 * (kk & 3),
                          sw128_desc(smem_u32(sK + (i & 1) * C::Tile + (kk >> 2) * C::Atom)) + 2 * (kk & 3), kIdescS, kk > 0);
-      umma_commit_warp(&sready[g]);
-      if (PAIR && g == groups - 1 && i + 2 < nb) umma_commit_warp(&kfree[i & 1]);
+      umma_commit_warp(&sready[b]);
+      if (PAIR && b == groups - 1 && i + 2 < nb) umma_commit_warp(&kfree[i & 1]);
     };
-    // accumulator of g += weights of block i . V, as the two halves of the weights come
-    auto weigh = [&](int g, int i, int done) {
-      const uint32_t d = tmem + C::ColO + g * C::StepO, p = tmem + C::ColP + g * C::StepP;
+    // accumulator of buffer b's group += weights of block i . V, as the two halves of the weights come
+    auto weigh = [&](int b, int i, int phase) {
+      const uint32_t d = tmem + C::ColO + (PAIR ? b * C::StepO : 0), p = tmem + b * 128;
       const uint64_t v = sw128_desc_mn(smem_u32(sV + (i & 1) * C::Tile), C::Atom);  // 16 keys are 2,048 B
-      const int steps = (min(kApTcKeys, j1 - j0 - i * kApTcKeys) + 15) / 16, phase = PAIR ? i : i >> 1;
+      const int steps = (min(kApTcKeys, j1 - j0 - i * kApTcKeys) + 15) / 16;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (!wait(&pready[2 * g + h], phase)) return false;
+        if (!wait(&pready[2 * b + h], phase)) return false;
         tc_fence_after();
         if (steps >= 4 * h + 4) {
 #pragma unroll
-          for (int kk = 4 * h; kk < 4 * h + 4; ++kk) umma_f16_ta_warp(d, p + kk * 8, v + kk * 128, kIdescO, i > 0 || kk > 0);
+          for (int kk = 4 * h; kk < 4 * h + 4; ++kk) {
+            umma_f16_ta_warp(d, p + (kk >> 1) * 32 + (kk & 1) * 8, v + kk * 128, kIdescO, i > 0 || kk > 0);
+            umma_f16_ta_warp(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + 16, v + kk * 128, kIdescO, 1);
+          }
         } else {  // the last block: steps of 16 keys past the range are left out
-          for (int kk = 4 * h; kk < steps; ++kk) umma_f16_ta_warp(d, p + kk * 8, v + kk * 128, kIdescO, i > 0 || kk > 0);
+          for (int kk = 4 * h; kk < steps; ++kk) {
+            umma_f16_ta_warp(d, p + (kk >> 1) * 32 + (kk & 1) * 8, v + kk * 128, kIdescO, i > 0 || kk > 0);
+            umma_f16_ta_warp(d, p + (kk >> 1) * 32 + (kk & 1) * 8 + 16, v + kk * 128, kIdescO, 1);
+          }
         }
       }
-      umma_commit_warp(&pvdone[done]);
-      if (PAIR && g == groups - 1 && i + 2 < nb) umma_commit_warp(&vfree[i & 1]);
+      umma_commit_warp(&pvdone[b]);
+      if (PAIR && b == groups - 1 && i + 2 < nb) umma_commit_warp(&vfree[i & 1]);
       return true;
     };
     bool ok = arrived(kfull, 0) && wait(qfull, 0);
@@ -211,7 +223,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ok = ok && arrived(vfull, 0);
       for (int i = 0; ok && i < nb; ++i)
         for (int g = 0; ok && g < groups; ++g) {
-          ok = weigh(g, i, g) && (g > 0 || arrived(kfull, i + 1));
+          ok = weigh(g, i, i) && (g > 0 || arrived(kfull, i + 1));
           if (!ok || i + 1 >= nb) continue;
           // the next scores overwrite the weights: wait until they have been used
           ok = wait(&pvdone[g], i);
@@ -223,13 +235,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       ok = ok && arrived(kfull, 1);
       if (ok && nb > 1) scores(1, 1);
       ok = ok && arrived(vfull, 0);
+      int b = 0, b2 = 2, phase = 0, before = 0;  // block i's buffer and phase, block i + 2's buffer, block i - 1's phase
       for (int i = 0; ok && i < nb; ++i) {
-        const int w = i & 1;
-        if (i + 2 < nb) {
-          ok = arrived(kfull, i + 2) && wait(&sread[w], i >> 1);
-          if (ok) scores(w, i + 2);
+        if (i + 2 < nb) {  // into the buffer of block i - 1, once its weights have been used
+          ok = arrived(kfull, i + 2) && (i == 0 || wait(&pvdone[b2], before));
+          if (ok) scores(b2, i + 2);
         }
-        ok = ok && weigh(w, i, i & 3) && arrived(vfull, i + 1);
+        ok = ok && weigh(b, i, phase) && arrived(vfull, i + 1);
+        b2 = b;
+        before = phase;
+        if (++b == 3) b = 0, ++phase;
       }
     }
     if (!ok) *failed = 1;
@@ -267,18 +282,19 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     if (lane == 0) mbar_arrive(qfull);
 
     const float scale = rsqrtf((float)HD) * 1.4426950408889634f;  // scores in powers of two
-    const uint32_t ts = tmem + lanes + grp * 128, tp = tmem + lanes + C::ColP + grp * C::StepP,
-                   to = tmem + lanes + C::ColO + grp * C::StepO;
+    const uint32_t to = tmem + lanes + C::ColO + grp * C::StepO;
     const int q = warp & 3;
     auto wait = [&](uint64_t* bar, int phase) {
       return __all_sync(0xffffffffu, mbar_wait_f(bar, (uint32_t)phase & 1, failed)) != 0;
     };
     // the product of block i with its V has ended
-    auto product = [&](int i) { return PAIR ? wait(&pvdone[grp], i) : wait(&pvdone[i & 3], i >> 2); };
+    auto product = [&](int i) { return PAIR ? wait(&pvdone[grp], i) : wait(&pvdone[i % 3], i / 3); };
     for (int k = 0; k < mine; ++k) {
       const int i = PAIR ? k : 2 * k + grp, keys = min(kApTcKeys, j1 - j0 - i * kApTcKeys);
       const int before = grp ? k : k - 1;  // the other group's last block before this one
-      if (!wait(&sready[grp], k)) {
+      const int buf = PAIR ? grp : i % 3;
+      const uint32_t ts = tmem + lanes + buf * 128;
+      if (!wait(&sready[buf], PAIR ? i : i / 3)) {
         *failed = 1;
         break;
       }
@@ -286,9 +302,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       uint32_t s[2][64];
       tmem_ld64(ts, s[0]);
       tmem_ld64(ts + 64, s[1]);
-      tc_fence_before();
-      __syncwarp();
-      if (!PAIR && lane == 0) mbar_arrive(&sread[grp]);
       if (keys < kApTcKeys) {
 #pragma unroll
         for (int e = 0; e < 128; ++e)
@@ -311,16 +324,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         refs[row] = now;
         __syncwarp();
         if (lane == 0) mbar_arrive(&refset[grp * 4 + q]);
-        if (k > 0 && !product(i - 2)) {  // frees the weights' buffer
-          *failed = 1;
-          break;
-        }
       }
       if (__any_sync(0xffffffffu, i > 0 && now != in)) {
         // This block moves the scale: every earlier product has to be in the accumulator. (With
-        // PAIR it is: these scores came after it. Otherwise, as a parity stands for one of two
-        // phases: the barrier's last one, four blocks back, ended before block i - 4's product,
-        // which this warp saw.)
+        // PAIR it is: these scores came after it. Otherwise block i - 1's may not be; its barrier's
+        // phase before, block i - 4's, has ended, as these scores came after block i - 3's product.)
         if (!PAIR && !product(i - 1)) {
           *failed = 1;
           break;
@@ -343,16 +351,22 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       bool good = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t p[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float p0 = ap_exp2(fmaf(__uint_as_float(s[h][2 * e]), scale, -off));
-          const float p1 = ap_exp2(fmaf(__uint_as_float(s[h][2 * e + 1]), scale, -off));
-          sum[(2 * e) & 3] += p0;
-          sum[(2 * e + 1) & 3] += p1;
-          p[e] = h2_bits(__floats2half2_rn(p0, p1));
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[32];  // hi terms of 32 keys, then their lo terms
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float p0 = ap_exp2(fmaf(__uint_as_float(s[h][32 * c + 2 * e]), scale, -off));
+            const float p1 = ap_exp2(fmaf(__uint_as_float(s[h][32 * c + 2 * e + 1]), scale, -off));
+            sum[(2 * e) & 3] += p0;
+            sum[(2 * e + 1) & 3] += p1;
+            const __half2 hi = __floats2half2_rn(p0, p1);
+            const float2 f = __half22float2(hi);
+            p[e] = h2_bits(hi);
+            p[16 + e] = h2_bits(__floats2half2_rn(p0 - f.x, p1 - f.y));
+          }
+          tmem_st32(ts + 64 * h + 32 * c, p);
         }
-        tmem_st32(tp + 32 * h, p);
         if (h == 0 && keys < kApTcKeys) {  // the V rows of the last step that lie past the range
           good = wait(&vfull[i & 1], i >> 1);
           if (!good) break;
@@ -365,7 +379,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pready[2 * grp + h]);
+        if (lane == 0) mbar_arrive(&pready[2 * buf + h]);
       }
       if (!good) {
         *failed = 1;

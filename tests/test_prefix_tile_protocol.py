@@ -179,6 +179,100 @@ def pair(m, nb, groups, slots_by_scores):
     return {"producer": producer(), "issuer": issuer(), **{f"group {g}": group(g) for g in range(groups)}}
 
 
+def single(m, nb, parity_buffers=False):
+    """Tiles of 128 rows: the groups take alternate blocks, whose scores and then weights lie in one of
+    three buffers in turn. parity_buffers: barriers and buffers by the block's parity instead (what the
+    kernel must not do: block i + 2's scores would overwrite weights in use)."""
+    nbuf = 2 if parity_buffers else 3
+    kfull, vfull = ([Barrier(f"{n}{i}") for i in range(2)] for n in ("kfull", "vfull"))
+    sready, pvdone = ([Barrier(f"{n}{b}") for b in range(nbuf)] for n in ("sready", "pvdone"))
+    pready = [[Barrier(f"pready{b}{h}") for h in range(2)] for b in range(nbuf)]
+    refset = [Barrier(f"refset{g}") for g in range(2)]
+    state = {"k": -1, "v": -1, "ref": -1}  # last block whose products have read K, V; that set the scale
+
+    def at(bars, i):
+        return bars[i % nbuf], i // nbuf
+
+    def producer():
+        def load_k(i):
+            if i >= 2:
+                yield at(sready, i - 2)
+                assert state["k"] >= i - 2
+            m.copy(("k", i & 1), i, kfull[i & 1])
+
+        def load_v(i):
+            if i >= 2:
+                yield at(pvdone, i - 2)
+                assert state["v"] >= i - 2
+            m.copy(("v", i & 1), i, vfull[i & 1])
+
+        yield from load_k(0)
+        for i in range(nb):
+            if i + 1 < nb:
+                yield from load_k(i + 1)
+            yield from load_v(i)
+
+    def issuer():
+        def scores(i):
+            m.product({("k", i & 1): i}, (("s", i % nbuf), ("scores", i)), [None, ("used", i - nbuf)])
+            m.commit(_Note(lambda: state.update(k=i)))
+            m.commit(sready[i % nbuf])
+
+        def weigh(i):
+            bar, phase = at(pready, i)
+            for h in range(2):
+                yield (bar[h], phase)
+                assert m.mem[("s", i % nbuf)] in ([("weights", i)] if h else [("half", i), ("weights", i)])
+                m.product({("v", i & 1): i}, ("o", (i, h)), [(i - 1, 1) if i else None] if h == 0 else [(i, 0)])
+            m.product({("s", i % nbuf): ("weights", i)}, (("s", i % nbuf), ("used", i)), [("weights", i)])
+            m.commit(_Note(lambda: state.update(v=i)))
+            m.commit(pvdone[i % nbuf])
+
+        yield (kfull[0], 0)
+        scores(0)
+        if nb > 1:
+            yield (kfull[1], 0)
+            scores(1)
+        yield (vfull[0], 0)
+        for i in range(nb):
+            if i + 2 < nb:
+                yield (kfull[(i + 2) & 1], (i + 2) >> 1)
+                if i > 0:
+                    yield at(pvdone, i - 1)
+                scores(i + 2)
+            yield from weigh(i)
+            if i + 1 < nb:
+                yield (vfull[(i + 1) & 1], (i + 1) >> 1)
+
+    def group(g):
+        mine = range(g, nb, 2)
+        for k, i in enumerate(mine):
+            yield at(sready, i)
+            assert m.mem[("s", i % nbuf)] == ("scores", i)
+            if i > 0:
+                yield (refset[1 - g], k if g else k - 1)
+            assert state["ref"] == i - 1
+            state["ref"] = i
+            refset[g].arrive()
+            if i > 0 and m.rng.random() < 0.5:  # the scale moves: every product before is in the accumulator
+                yield at(pvdone, i - 1)
+                assert m.mem["o"] == (i - 1, 1)
+            m.put(("s", i % nbuf), ("half", i), [("scores", i)])
+            bar, _ = at(pready, i)
+            bar[0].arrive()
+            yield from pause()
+            if i == nb - 1:
+                yield (vfull[i & 1], i >> 1)
+                assert m.mem[("v", i & 1)] == i
+            m.put(("s", i % nbuf), ("weights", i), [("half", i)])
+            bar[1].arrive()
+        if len(mine):
+            yield at(pvdone, mine[-1])
+            assert state["v"] >= mine[-1]
+
+    return {"producer": producer(), "issuer": issuer(), "group 0": group(0), "group 1": group(1)}
+
+
 class _Note:
     """Something noted when the products before it have ended."""
 
@@ -198,6 +292,25 @@ def test_tiles_of_256_rows(nb, groups):
     for seed in range(150):
         m = Model(random.Random(1000 * nb + seed))
         m.run(pair(m, nb, groups, False))
+
+
+@pytest.mark.parametrize("nb", [1, 2, 3, 4, 5, 6, 7, 8, 13])
+def test_tiles_of_128_rows(nb):
+    for seed in range(300):
+        m = Model(random.Random(5000 * nb + seed))
+        m.run(single(m, nb))
+
+
+def test_the_model_sees_too_few_buffers():
+    """Two buffers for three blocks under way: overwritten weights, or a wait that is late or early."""
+    wrong = 0
+    for seed in range(300):
+        m = Model(random.Random(seed))
+        try:
+            m.run(single(m, 8, True))
+        except AssertionError:
+            wrong += 1
+    assert wrong > 0
 
 
 def test_the_model_sees_a_barrier_that_passes_every_block():
