@@ -816,11 +816,15 @@ struct ApPlan {
 };
 
 constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V heads, keys of a row: one launch
-// Query rows of a unit, and blocks of 128 x 128 (rows, keys) over all heads, from which the prefix
-// takes the tcgen05 tiles. A third launch and their start cost ~5 us: 16 rows x 8 heads x 4 behind
-// 2,048 entries (128 blocks) 16.5 us with them, 12.0 without; 64 x 32 heads behind 512 (128 blocks)
-// 25.2 and 24.7, behind 1,024 26.1 and 28.0, behind 4,096 65.8 and 80.
-constexpr int kApTcFrom = 32, kApTcBlocks = 256;
+// The tcgen05 tiles take the prefix where units have more than 32 query rows and there are 256 blocks
+// of 128 x 128 (query rows, keys) over all heads, or where units have more than 16 (a tile is then
+// mostly empty) and 1,024 blocks. A third launch and their start cost ~5 us: 16 rows x 8 heads x 4
+// behind 2,048 entries (64 query rows, 128 blocks) 18.8 us with them, 13.6 without; 64 x 32 heads
+// behind 512 (128 blocks) 24.8 and 23.2, behind 1,024 27.9 and 26.9, behind 4,096 37.6 and 51.6; 64 x 8
+// x 4 behind 2,048 (256 blocks of 256 query rows) 28.4 and 29.3. 32 rows x 32 heads behind 1,024
+// (256 blocks) 21.6 and 20.2, behind 4,096 (1,024) 33.6 and 37.2; two units of them behind 1,024 (512)
+// 28.7 and 26.2, behind 2,048 (1,024) 34.3 and 36.3. 16 units of 8 x 32 heads behind 1,024: 84.8 and 57.8.
+constexpr int kApTcRowsFrom = 32, kApTcBlocks = 256, kApTcFewFrom = 16, kApTcFewBlocks = 1024;
 // Own entries of a row up to which single warps take them, where their warps (two per SM or more)
 // fill the SMs, and up to which they always do. 64 x 32 heads of up to 64, 128 and 256 entries: 14.1,
 // 20.6 and 35.8 us by warps, 22.0, 26.5 and 35.8 by tiles; 4 x 8 heads x 4 of up to 256: 11.2 and
@@ -833,10 +837,13 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
                uint32_t max_own, int track) {
   ApPlan p;
   p.G = (int)(nh / nkv);
-  const int rows_p = (int)std::min<uint32_t>(M, kApMaxUnitRows) * p.G;
+  // query rows of a unit, as if all were as large
   const bool some = num_units > 0 && max_prefix > 0;
-  p.tc = some && hd != 32 && rows_p > kApTcFrom &&
-         nkv * (((size_t)M * p.G + 127) / 128) * ((max_prefix + 127) / 128) >= (size_t)kApTcBlocks;
+  const int rows_p = (int)std::min<uint32_t>(some ? (uint32_t)(((uint64_t)M + num_units - 1) / num_units) : M, kApMaxUnitRows) * p.G;
+  const size_t blocks_k = nkv * (size_t)((max_prefix + 127) / 128);
+  p.tc = some && hd != 32 &&
+         ((rows_p > kApTcRowsFrom && blocks_k * (((size_t)M * p.G + 127) / 128) >= (size_t)kApTcBlocks) ||
+          (rows_p > kApTcFewFrom && blocks_k * num_units >= (size_t)kApTcFewBlocks));
   p.blk_p = p.tc ? kApTcKeys : kApKeys;
   p.wr_p = std::min(ap_wr(rows_p), hd == 32 || p.G > 32 ? 4 : 2);  // 64 rows of 64 or 128 dims spill
   p.wr_o = ap_wr(p.G);
