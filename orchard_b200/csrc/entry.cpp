@@ -17,40 +17,48 @@ namespace {
 
 PyObject* g_data_ptr = nullptr;  // "data_ptr"
 
-// Any whole number; a Python error and 0 otherwise.
-unsigned long long whole(PyObject* o) {
+// Conversions. `ok` turns false with a Python error set; from then on nothing more is asked of the
+// arguments (a call into Python with an error set would replace it by a SystemError).
+unsigned long long whole(PyObject* o, bool& ok) {
   if (PyLong_Check(o)) return PyLong_AsUnsignedLongLongMask(o);
   PyObject* i = PyNumber_Index(o);
-  if (i == nullptr) return 0;
+  ok = i != nullptr;
+  if (!ok) return 0;
   const unsigned long long v = PyLong_AsUnsignedLongLongMask(i);
   Py_DECREF(i);
   return v;
 }
 
-unsigned long long address(PyObject* o) {
+unsigned long long address(PyObject* o, bool& ok) {
   if (o == Py_None) return 0;
   if (PyLong_Check(o)) return PyLong_AsUnsignedLongLongMask(o);
   PyObject* p = PyObject_CallMethodNoArgs(o, g_data_ptr);
-  if (p == nullptr) return 0;
-  const unsigned long long v = whole(p);
+  ok = p != nullptr;
+  if (!ok) return 0;
+  const unsigned long long v = whole(p, ok);
   Py_DECREF(p);
   return v;
 }
 
 template <typename T>
-T convert(PyObject* o) {
-  if constexpr (std::is_pointer_v<T>)
-    return reinterpret_cast<T>(static_cast<uintptr_t>(address(o)));
-  else if constexpr (std::is_floating_point_v<T>)
-    return static_cast<T>(PyFloat_AsDouble(o));
-  else
-    return static_cast<T>(whole(o));
+T convert(PyObject* o, bool& ok) {
+  if (!ok) return T{};
+  if constexpr (std::is_pointer_v<T>) {
+    return reinterpret_cast<T>(static_cast<uintptr_t>(address(o, ok)));
+  } else if constexpr (std::is_floating_point_v<T>) {
+    const double v = PyFloat_AsDouble(o);
+    ok = v != -1.0 || PyErr_Occurred() == nullptr;
+    return static_cast<T>(v);
+  } else {
+    return static_cast<T>(whole(o, ok));
+  }
 }
 
 template <typename... A, size_t... I>
 PyObject* invoke(int (*fn)(A...), PyObject* const* args, std::index_sequence<I...>) {
-  const std::tuple<A...> v{convert<A>(args[I])...};  // braces: converted in order
-  if (PyErr_Occurred()) return nullptr;
+  bool ok = true;
+  const std::tuple<A...> v{convert<A>(args[I], ok)...};  // braces: converted in order
+  if (!ok) return nullptr;
   int status = 0;
   Py_BEGIN_ALLOW_THREADS;
   status = fn(std::get<I>(v)...);
