@@ -318,7 +318,8 @@ int orch_embed_rows(const int32_t* ids, const void* table, int table_dt, float* 
  * A row whose slot or length is out of range, whose unit is, or that is in two units, is not
  * written (nor its mass) and sets device check bit 8 (slot) / 2; where units overlap, so may be
  * rows of the units after them. `workspace`, 16-byte aligned, holds
- * orch_attention_prefix_workspace_bytes() bytes (the same arguments; track: mass given). */
+ * orch_attention_prefix_workspace_bytes() bytes (the same arguments; track: mass given). q, out,
+ * caches, prefixes and units are 16-byte aligned, other buffers for their elements. */
 size_t orch_attention_prefix_workspace_bytes(uint32_t M, uint32_t num_heads, uint32_t num_kv_heads,
                                              uint32_t head_dim, uint32_t num_units, uint32_t max_prefix,
                                              uint32_t max_own, int track);
@@ -368,7 +369,7 @@ int orch_cache_evict(void* k_cache, void* v_cache, const float* mass, const int3
  *   int32 [M + 1]): l += the bias of v, the last one if v is listed twice. NULL: none;
  *   masks uint32 [num_masks, mask_words], row m's is mask_rows[m] (negative: none): l = -inf
  *   unless bit v & 31 of word v >> 5 is set (ids past the words are not allowed). NULL: none.
- * Ids outside the slice are skipped. A row whose hist_len, bias range or mask index is out of
+ * Ids outside the slice are skipped. Buffers are aligned for their elements. A row whose hist_len, bias range or mask index is out of
  * range is not written and sets device check bit 16. */
 int orch_logits_process(const void* logits, void* out, int dt, uint32_t M, uint32_t V, uint32_t ld, uint32_t base,
                         const int32_t* history, uint32_t history_ld, const int32_t* hist_len,

@@ -998,6 +998,8 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   ORCH_REQUIRE((((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)out | (uintptr_t)prefix_k |
                  (uintptr_t)prefix_v | (uintptr_t)units | (uintptr_t)workspace) & 15) == 0,
                "attention_prefix: buffers must be 16-byte aligned");
+  ORCH_REQUIRE((((uintptr_t)lens | (uintptr_t)slots | (uintptr_t)mass) & 3) == 0,
+               "attention_prefix: lens, slots and mass must be 4-byte aligned");
   if (!ap_shape_ok(M, num_heads, num_kv_heads, head_dim))
     return fail(ORCH_ERR_UNSUPPORTED, "attention_prefix: too many rows and heads");
   const ApPlan p = ap_plan(M, num_heads, num_kv_heads, head_dim, num_units, max_prefix, max_own, mass != nullptr);

@@ -453,6 +453,9 @@ extern "C" int orch_cache_evict(void* k_cache, void* v_cache, const float* mass,
   ORCH_REQUIRE(num_kv_heads > 0 && max_seq > 0 && num_slots > 0 && num_slots <= 0x7fffffffu, "cache_evict: empty shape");
   ORCH_REQUIRE(head_dim > 0 && head_dim % 8 == 0 && head_dim <= 1024, "cache_evict: head_dim must be a multiple of 8, at most 1024");
   ORCH_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, "cache_evict: caches must be 16-byte aligned");
+  ORCH_REQUIRE((((uintptr_t)mass | (uintptr_t)positions | (uintptr_t)lens | (uintptr_t)slots | (uintptr_t)mass_out |
+                 (uintptr_t)positions_out | (uintptr_t)lens_out) & 3) == 0,
+               "cache_evict: mass, positions, lens and slots must be 4-byte aligned");
   ORCH_REQUIRE(lens_out != lens, "cache_evict: lens_out must not be lens (heads read it while others finish)");
   ORCH_REQUIRE((mass_out == mass) == (positions_out == positions),
                "cache_evict: mass and positions are both updated in place, or neither");

@@ -418,7 +418,7 @@ extern "C" int orch_q4t_qkv_rope_at(const void* tiled_qkv, const void* x, uint32
                                     const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
                                     void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots,
                                     const float* lora_t, const float* lora_b, uint32_t lora_r, void* stream) {
-  ORCH_REQUIRE(M == 0 || index, "q4t_qkv_rope_at: null index");
+  ORCH_REQUIRE(M == 0 || (index && ((uintptr_t)index & 3) == 0), "q4t_qkv_rope_at: null or unaligned index");
   return qkv_rope(tiled_qkv, nullptr, true, x, M, K, H, num_heads, pos, index, slots, cos_tab, sin_tab, max_pos, q_out,
                   k_cache, v_cache, max_seq, num_slots, lora_t, lora_b, lora_r, stream);
 }
@@ -494,7 +494,7 @@ extern "C" int orch_q4t_rms_qkv_rope_at(const void* tiled_qkv, const float* x, c
                                         const float* cos_tab, const float* sin_tab, uint32_t max_pos, void* q_out,
                                         void* k_cache, void* v_cache, uint32_t max_seq, uint32_t num_slots,
                                         void* stream) {
-  ORCH_REQUIRE(M == 0 || index, "q4t_rms_qkv_rope_at: null index");
+  ORCH_REQUIRE(M == 0 || (index && ((uintptr_t)index & 3) == 0), "q4t_rms_qkv_rope_at: null or unaligned index");
   return rms_qkv_rope(tiled_qkv, x, norm_w, eps, xn, M, K, H, num_heads, pos, index, slots, cos_tab, sin_tab, max_pos,
                       q_out, k_cache, v_cache, max_seq, num_slots, stream);
 }

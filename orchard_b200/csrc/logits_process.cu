@@ -223,7 +223,7 @@ int lp_dispatch(const LpArgs& a, cudaStream_t st) {
   constexpr int V16 = 16 / sizeof(T);
   const bool wide = a.hist_ld > kLpPackedHist || a.num_bias > kLpPackedBias;
   // rows need not begin on 16 bytes, as long as in and out lie alike
-  const bool vec = (((uintptr_t)a.in ^ (uintptr_t)a.out) & 15) == 0 && (uintptr_t)a.in % sizeof(T) == 0;
+  const bool vec = (((uintptr_t)a.in ^ (uintptr_t)a.out) & 15) == 0;
   if (vec) return wide ? lp_launch<T, V16, true>(a, st) : lp_launch<T, V16, false>(a, st);
   return wide ? lp_launch<T, 1, true>(a, st) : lp_launch<T, 1, false>(a, st);
 }
@@ -253,6 +253,11 @@ extern "C" int orch_logits_process(const void* logits, void* out, int dt, uint32
   ORCH_REQUIRE(!masks || (mask_rows && mask_words > 0 && mask_words <= 0x4000000u && num_masks <= 0x7fffffffu),
                "logits_process: masks need mask_rows and mask_words");
   ORCH_REQUIRE(M <= 65535, "logits_process: at most 65,535 rows");
+  ORCH_REQUIRE((((uintptr_t)logits | (uintptr_t)out) & (dt == ORCH_F32 ? 3 : 1)) == 0 &&
+                   (((uintptr_t)history | (uintptr_t)hist_len | (uintptr_t)gen_start | (uintptr_t)penalties |
+                     (uintptr_t)bias_ids | (uintptr_t)bias_vals | (uintptr_t)bias_off | (uintptr_t)masks |
+                     (uintptr_t)mask_rows) & 3) == 0,
+               "logits_process: buffers must be aligned for their elements");
   LpArgs a;
   a.in = logits;
   a.out = out;
