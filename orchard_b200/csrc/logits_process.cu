@@ -32,6 +32,8 @@ constexpr int kLpMaxSlice = kLpThreads * kLpEach * kLpRounds;
 // bias entry + 1 (16 bits). Histories or bias lists too long for that take two words:
 // occurrences and seen, and the bias entry.
 constexpr int kLpPackedHist = 32767, kLpPackedBias = 65534;
+// Ids of a list at most: the loops over it count up to 4 x kLpThreads past its end.
+constexpr uint32_t kLpMaxList = 0x7fff0000u;
 
 struct LpArgs {
   const void* in;
@@ -246,10 +248,10 @@ extern "C" int orch_logits_process(const void* logits, void* out, int dt, uint32
   ORCH_REQUIRE(dt == ORCH_F32 || dt == ORCH_F16, "logits_process: bad dtype");
   ORCH_REQUIRE(ld >= V && ld <= 0x7fffffffu && (uint64_t)base + V <= 0x7fff0000u,
                "logits_process: row stride below V or too large, or ids out of range");
-  ORCH_REQUIRE((history == nullptr) == (penalties == nullptr) && (!history || (hist_len && history_ld <= 0x7fffffffu)),
-               "logits_process: penalties need history and hist_len (and history penalties)");
-  ORCH_REQUIRE(!bias_ids || (bias_vals && bias_off && num_bias <= 0x7fffffffu),
-               "logits_process: bias_ids need bias_vals and bias_off");
+  ORCH_REQUIRE((history == nullptr) == (penalties == nullptr) && (!history || (hist_len && history_ld <= kLpMaxList)),
+               "logits_process: penalties need history and hist_len (and history penalties), or history_ld is too large");
+  ORCH_REQUIRE(!bias_ids || (bias_vals && bias_off && num_bias <= kLpMaxList),
+               "logits_process: bias_ids need bias_vals and bias_off, or num_bias is too large");
   ORCH_REQUIRE(!masks || (mask_rows && mask_words > 0 && mask_words <= 0x4000000u && num_masks <= 0x7fffffffu),
                "logits_process: masks need mask_rows and mask_words");
   ORCH_REQUIRE(M <= 65535, "logits_process: at most 65,535 rows");

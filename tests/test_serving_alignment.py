@@ -36,3 +36,10 @@ def test_projections_refuse_an_unaligned_index():
     assert b"index" in L.orch_last_error()
     assert L.orch_q4t_rms_qkv_rope_at(P, P, P, 1e-5, P, 1, 256, 256, 4, P, P + 1, None, P, P, 8, P, P, P, 8, 1, None) == 1
     assert b"index" in L.orch_last_error()
+
+
+@pytest.mark.parametrize("size", [2 ** 31 - 1, 2 ** 31 - 65535])
+def test_logits_refuse_lists_past_what_a_loop_counts(size):
+    """A list's index is a 32-bit number that goes on by up to 2,048 past its end."""
+    assert logits(hist=P, hl=size, hn=P, pen=P) == 1 and b"history" in _lib.lib().orch_last_error()
+    assert logits(bi=P, bv=P, bo=P, nb=size) == 1 and b"bias" in _lib.lib().orch_last_error()
