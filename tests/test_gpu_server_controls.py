@@ -69,3 +69,34 @@ def test_biases_that_leave_nothing_are_reported(small):  # noqa: F811
     with pytest.raises(RuntimeError, match="32"):
         serving.BatchServer(llm).generate([[5, 6, 7], [8]], max_tokens=2, ignore_eos=True,
                                           controls=serving.LogitsControls(bias={v: float("-inf") for v in range(300)}))
+
+
+@pytest.mark.parametrize("hidden,heads,rows", [(512, 16, 6), (1024, 8, 12)])
+def test_batches_of_many_heads_give_the_engine_s_own_tokens(hidden, heads, rows):
+    """Rows x heads above 64, with and without the prompts' common beginning held apart: the tokens
+    of generate_batch_ids, as far as its logits tell two tokens apart (1e-3 of the largest; both
+    sides round fp16 activations in another order)."""
+    cfg = dict(hidden_size=hidden, num_attention_heads=heads, intermediate_size=512, num_hidden_layers=2, vocab_size=300,
+               rms_norm_eps=1e-5, max_position_embeddings=512)
+    _, raw = om.random_model(cfg, seed=6)
+    llm = Llama(checkpoint=from_tensors(cfg, hf_tensors(raw, 2)), max_batch=rows, max_seq=160)
+    g = np.random.default_rng(hidden)
+    head = g.integers(3, 300, 40).tolist()
+    tails = [g.integers(3, 300, 3 + 5 * i).tolist() for i in range(rows)]
+    whole = [head + t for t in tails]
+    steps = 10
+    want = llm.generate_batch_ids(whole, max_tokens=steps, temperature=0, ignore_eos=True)
+    for srv, prompts in ((serving.BatchServer(llm), whole), (serving.BatchServer(llm, prefix=head), tails)):
+        got = srv.generate(prompts, max_tokens=steps, ignore_eos=True)
+        for n in range(1, steps + 1):  # a row is compared up to its first difference
+            if all(got[b][:n] == want[b][:n] for b in range(rows)):
+                continue
+            llm.generate_batch_ids(whole, max_tokens=n, temperature=0, ignore_eos=True)
+            lg = llm.engine.logits[:rows].cpu().numpy()
+            for b in range(rows):
+                if got[b][:n] != want[b][:n] and got[b][:n - 1] == want[b][:n - 1]:
+                    assert lg[b, want[b][n - 1]] - lg[b, got[b][n - 1]] <= 1e-3 * np.abs(lg[b]).max(), (b, n)
+        llm.generate_batch_ids(whole, max_tokens=1, temperature=0, ignore_eos=True)
+        first = llm.engine.logits[:rows].cpu().numpy().copy()
+        srv.generate(prompts, max_tokens=1, ignore_eos=True)
+        assert rel_err(llm.engine.logits[:rows].cpu().numpy(), first) <= 2e-3
