@@ -290,7 +290,8 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
       if (d == 0) a.stat[mh * S + split] = make_float2(mx, l);
     }
   }
-  if (a.direct && keys.srow != nullptr) {  // the only row: its own entries' weights (n is G here)
+  // the only row (attn_prefix_row_kernel): its own entries' weights (n is G here)
+  if (a.direct && keys.srow != nullptr) {
     __syncthreads();  // scores written; O no longer needed
     float2* tot = reinterpret_cast<float2*>(ap_smem);
     if (tid < n) {
@@ -302,7 +303,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
       tot[tid] = make_float2(mx == -INFINITY ? 0.f : mx - kApShift, l == 0.f ? 0.f : 1.0f / l);
     }
     __syncthreads();
-    const int len = keys.own2 ? keys.n2 : keys.j1;
+    const int len = keys.n2;
     float* mass = a.mass + ((size_t)(a.slots ? a.slots[m0] : m0) * a.nkv + kv) * a.max_seq;
     for (int e = tid; e < len; e += 128) {
       float w = 0.f;
@@ -315,7 +316,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 // The same tile for one warp: the G <= 16 heads of a K/V head of row m over the row's own entries
 // [j0, j1), 16 keys at a time through the warp's own ring of two stages. Where there are enough
 // rows and heads, four of these per CTA need no barrier and no join across warps, and a quarter of
-// the CTAs: AAA.
+// the CTAs (measured at kApWarpKeys).
 template <int HD>
 __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __half* k, const __half* v, int j0, int j1,
                                         int split, float* srow) {
@@ -940,9 +941,9 @@ int ap_launch_shape(ApArgs a, cudaStream_t st) {
 // A tile of a unit has at least the rows of a tile of one row, so wr_p >= wr_o; with head_dim 64
 // or 128 it has 64 rows only where a row's heads already fill that.
 template <int HD>
-int ap_launch(const ApArgs& a, cudaStream_t st) {
-  const int p = a.tc || a.row || a.blocks_p == 0 ? 0 : a.wr_p;
-  const int o = a.by_warp ? 0 : a.wr_o;
+int ap_launch(const ApArgs& a, const ApPlan& plan, cudaStream_t st) {
+  const int p = a.tc || a.row || a.blocks_p == 0 ? 0 : plan.wr_p;
+  const int o = plan.by_warp ? 0 : plan.wr_o;
   if (p == 0)
     return o == 0 ? ap_launch_shape<HD, 0, 0>(a, st) : o == 1 ? ap_launch_shape<HD, 0, 1>(a, st)
          : o == 2 ? ap_launch_shape<HD, 0, 2>(a, st) : ap_launch_shape<HD, 0, 4>(a, st);
@@ -1027,8 +1028,6 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.nh = (int)num_heads;
   a.nkv = (int)num_kv_heads;
   a.G = p.G;
-  a.wr_p = p.wr_p;
-  a.wr_o = p.wr_o;
   a.tiles_p = p.tiles_p;
   a.tiles_o = p.tiles_o;
   a.S_p = p.S_p;
@@ -1045,7 +1044,6 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   a.blocks_p = (int)blocks_p;
   a.direct = p.direct;
   a.row = p.row;
-  a.by_warp = p.by_warp;
   a.acc = static_cast<float*>(workspace);
   a.stat = reinterpret_cast<float2*>(a.acc + p.acc_floats);
   a.scores = a.acc + p.acc_floats + p.stat_floats;
@@ -1053,8 +1051,8 @@ extern "C" int orch_attention_prefix(const void* q, const void* prefix_k, const 
   ORCH_CHECK_WORD(a.check);
   cudaStream_t st = as_stream(stream);
   switch (head_dim) {
-    case 32: return ap_launch<32>(a, st);
-    case 64: return ap_launch<64>(a, st);
-    default: return ap_launch<128>(a, st);
+    case 32: return ap_launch<32>(a, p, st);
+    case 64: return ap_launch<64>(a, p, st);
+    default: return ap_launch<128>(a, p, st);
   }
 }

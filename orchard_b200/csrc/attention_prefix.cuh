@@ -26,7 +26,6 @@ struct ApArgs {
   float* mass;
   __half* out;
   int M, nh, nkv, G;
-  int wr_p, wr_o;        // warps along the rows of a prefix tile / an own tile
   int tr_p, tr_sh;       // query rows of a prefix tile, and their logarithm
   int tiles_p, tiles_o;  // row tiles of all units (as many as disjoint ones can have) / per row
   int S_p, S_o;          // key ranges of a prefix / of a row's own entries
@@ -34,7 +33,6 @@ struct ApArgs {
   int tc;                // the prefix part runs in its own kernel (attention_prefix_tc.cu)
   int blocks_p;          // CTAs of the prefix part
   int row;               // few rows and keys: a CTA per row and K/V head takes all of them
-  int by_warp;           // own entries by single warps, four rows and K/V heads per CTA
   int direct;            // the output is written by the attention kernel: nothing to join
   float* acc;            // [M * nh][S][HD]
   float2* stat;          // [M * nh][S]: (max, sum), in powers of two

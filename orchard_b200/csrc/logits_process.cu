@@ -9,13 +9,14 @@
 //   l = -inf where the row's mask has bit v clear
 //
 // Bound by memory: every logit is read and written once. A CTA takes a slice of one row's
-// vocabulary, requests the whole slice (16 logits per thread) before anything else, and while
-// those loads are in flight counts the row's history into a table of the slice in shared memory
-// (integer atomics: the result has no order). A slice is as small as keeps the grid within one
-// round of CTAs, so that few rows still use many SMs; wide batches take the largest slice, two
-// rounds of loads, where the history is read least often (128 rows x 131,072 with 4,095 ids of
-// history: 37 us, 42 us with slices of one round, 24 us with no control at all; sharing the
-// history over a cluster's tables took 93 us, its distributed-shared-memory atomics being slow).
+// vocabulary, requests it (16 logits per thread; in wide batches the first half of it) before
+// anything else, and while those loads are in flight counts the row's history into a table of the
+// slice in shared memory (integer atomics: the result has no order). A slice is as small as keeps
+// the grid within one round of CTAs, so that few rows still use many SMs; wide batches take the
+// largest slice, two rounds of loads, where the history is read least often (128 rows x 131,072
+// with 4,095 ids of history: 37 us, 42 us with slices of one round, 24 us with no control at all;
+// sharing the history over a cluster's tables took 93 us, its distributed-shared-memory atomics
+// being slow).
 #include <algorithm>
 
 #include "orch_common.cuh"
