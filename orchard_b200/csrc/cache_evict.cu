@@ -480,13 +480,14 @@ extern "C" int orch_cache_evict(void* k_cache, void* v_cache, const float* mass,
   a.recent = recent;
   ORCH_CHECK_WORD(a.check);
   const size_t bits = ((size_t)max_seq + 127) / 128 * 16, staged = bits + ((size_t)max_seq + 3) / 4 * 16;
-  // CTAs per (row, head): two while they fit in two rounds of two per SM (rows that lose nothing
-  // leave at once; 32 rows x 8 heads of up to 1,537 entries: 15.1 us, 17.1 with one), more while
-  // they run at once (4 x 32 heads of 16,384 entries: 92 us with two, 101 with four), each with at
-  // least 128 moves (a step of one entry: 8.6 us with one, 19 with two)
+  // CTAs per (row, head): twice as many while all of them run at once, two per SM (8 x 32 heads,
+  // 1,024 -> 512: 23.7 us with one, 32.3 with two, which no longer do; 9 x 32, 2,048 -> 1,024: 41.6 and
+  // 47.6; 4 x 32, 16,384 -> 4,096: 96.8 with two, 109.6 with four. Rows that lose nothing leave at once,
+  // which the host cannot see: 32 x 8 heads of 1 to 1,537 -> 1,024 take 17.4 with one, 15.4 with two),
+  // each with at least 128 moves (a step of one entry: 8.6 us with one, 19 with two)
   const uint32_t pairs = M * num_kv_heads, most = std::min<uint32_t>(a.budget, max_seq - a.budget);
   uint32_t c = 1;
-  while (c < 8 && 2 * c * (uint64_t)pairs <= (c == 1 ? 4u : 2u) * (uint64_t)num_sms() && most >= 256 * c) c *= 2;
+  while (c < 8 && c * (uint64_t)pairs <= (uint64_t)num_sms() && most >= 256 * c) c *= 2;
   a.cluster = (int)c;
   if ((uint64_t)pairs * c > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "cache_evict: too many rows and heads");
   return staged <= (size_t)kEvStaged ? ev_launch<512, true>(a, staged, as_stream(stream))
