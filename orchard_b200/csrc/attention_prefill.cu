@@ -45,21 +45,6 @@ struct PfArgs {
 __device__ __forceinline__ uint32_t ld_h2(const __half* p) { return *reinterpret_cast<const uint32_t*>(p); }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) { return h2_bits(__floats2half2_rn(lo, hi)); }
 
-__device__ __forceinline__ void pf_cp16(const void* dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
-               "l"(src), "r"(ok ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void ldsm_x4(const __half* p, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
-}
-__device__ __forceinline__ void ldsm_x4_t(const __half* p, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
-}
 
 __global__ void __launch_bounds__(128, 3) attn_prefill_kernel(const PfArgs a) {
   extern __shared__ __align__(16) uint8_t pf_smem[];
@@ -93,8 +78,8 @@ __global__ void __launch_bounds__(128, 3) attn_prefill_kernel(const PfArgs a) {
       const int i = tid + 128 * j, r = i >> 4, d8 = (i & 15) * 8, key = kb * kPfKeys + r;
       const bool ok = key <= plast;
       const size_t off = ok ? base + (size_t)key * kPfHD + d8 : 0;
-      pf_cp16(kd + r * kPfP + d8, a.kc + off, ok);
-      pf_cp16(vd + r * kPfP + d8, a.vc + off, ok);
+      cp_async16(kd + r * kPfP + d8, a.kc + off, ok);
+      cp_async16(vd + r * kPfP + d8, a.vc + off, ok);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -150,7 +135,7 @@ __global__ void __launch_bounds__(128, 3) attn_prefill_kernel(const PfArgs a) {
 #pragma unroll
       for (int kk = 0; kk < kPfHD / 16; kk += 2) {
         uint32_t b[4];
-        ldsm_x4(ks + (8 * t + lr) * kPfP + 16 * kk + 8 * lm, b);
+        ldmatrix4(ks + (8 * t + lr) * kPfP + 16 * kk + 8 * lm, b);
         mma_16816(sc[t], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], b[0], b[1]);
         mma_16816(sc[t], qa[kk + 1][0], qa[kk + 1][1], qa[kk + 1][2], qa[kk + 1][3], b[2], b[3]);
       }
@@ -220,7 +205,7 @@ __global__ void __launch_bounds__(128, 3) attn_prefill_kernel(const PfArgs a) {
 #pragma unroll
       for (int d = 0; d < kPfHD / 8; d += 2) {
         uint32_t b[4];
-        ldsm_x4_t(vs + (16 * j + 8 * (lm & 1) + lr) * kPfP + 8 * d + 8 * (lm >> 1), b);
+        ldmatrix4_t(vs + (16 * j + 8 * (lm & 1) + lr) * kPfP + 8 * d + 8 * (lm >> 1), b);
         mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
         mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
         mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);

@@ -32,21 +32,6 @@ namespace orch {
 
 namespace {
 
-__device__ __forceinline__ void ap_cp16(void* dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
-               "l"(src), "r"(ok ? 16 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void ap_ldsm4(const __half* p, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
-}
-__device__ __forceinline__ void ap_ldsm4_t(const __half* p, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))));
-}
 // Half-element offset of 16-byte piece c of row r in a tile of HD-wide rows: pieces are permuted
 // within 128 bytes so that the eight rows of an ldmatrix fall in distinct banks.
 template <int HD>
@@ -96,8 +81,8 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
     for (int j = 0; j < kApKeys / RS; ++j) {
       const bool ok = j * RS < left;
       const int step = ok ? j * RS * HD : 0;  // rows past the end are filled with zeros, not read
-      ap_cp16(kd + j * RS * HD, kb + step, ok);
-      ap_cp16(kd + TILE + j * RS * HD, vb + step, ok);
+      cp_async16(kd + j * RS * HD, kb + step, ok);
+      cp_async16(kd + TILE + j * RS * HD, vb + step, ok);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -152,7 +137,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 #pragma unroll
       for (int kk = 0; kk < HD / 16; kk += 2) {
         uint32_t bb[4];
-        ap_ldsm4(ks + ap_at<HD>(8 * (kt0 + t) + lr, 2 * kk + lm), bb);
+        ldmatrix4(ks + ap_at<HD>(8 * (kt0 + t) + lr, 2 * kk + lm), bb);
         mma_16816(sc[t], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bb[0], bb[1]);
         mma_16816(sc[t], qa[kk + 1][0], qa[kk + 1][1], qa[kk + 1][2], qa[kk + 1][3], bb[2], bb[3]);
       }
@@ -227,7 +212,7 @@ __device__ __forceinline__ void ap_tile(const ApArgs& a, int m0, int i0, int n, 
 #pragma unroll
       for (int d = 0; d < HD / 8; d += 2) {
         uint32_t bb[4];
-        ap_ldsm4_t(vs + ap_at<HD>(8 * kt0 + 16 * j + 8 * (lm & 1) + lr, d + (lm >> 1)), bb);
+        ldmatrix4_t(vs + ap_at<HD>(8 * kt0 + 16 * j + 8 * (lm & 1) + lr, d + (lm >> 1)), bb);
         mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], bb[0], bb[1]);
         mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], bb[2], bb[3]);
         mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
@@ -334,8 +319,8 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
     for (int j = 0; j < KEYS / RS; ++j) {
       const bool ok = j * RS < left;
       const int step = ok ? j * RS * HD : 0, at = ap_at<HD>(r0 + j * RS, c8);  // past the end: zeros, not read
-      ap_cp16(kd + at, k + off + step, ok);
-      ap_cp16(kd + TILE + at, v + off + step, ok);
+      cp_async16(kd + at, k + off + step, ok);
+      cp_async16(kd + TILE + at, v + off + step, ok);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -374,7 +359,7 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
 #pragma unroll
       for (int kk = 0; kk < HD / 16; kk += 2) {
         uint32_t bb[4];
-        ap_ldsm4(ks + ap_at<HD>(8 * t + lr, 2 * kk + lm), bb);
+        ldmatrix4(ks + ap_at<HD>(8 * t + lr, 2 * kk + lm), bb);
         mma_16816(sc[t], qa[kk][0], qa[kk][1], qa[kk][2], qa[kk][3], bb[0], bb[1]);
         mma_16816(sc[t], qa[kk + 1][0], qa[kk + 1][1], qa[kk + 1][2], qa[kk + 1][3], bb[2], bb[3]);
       }
@@ -435,7 +420,7 @@ __device__ __forceinline__ void ap_warp(const ApArgs& a, int m, int kv, const __
 #pragma unroll
     for (int d = 0; d < HD / 8; d += 2) {
       uint32_t bb[4];
-      ap_ldsm4_t(vs + ap_at<HD>(8 * (lm & 1) + lr, d + (lm >> 1)), bb);
+      ldmatrix4_t(vs + ap_at<HD>(8 * (lm & 1) + lr, d + (lm >> 1)), bb);
       mma_16816(o[d], hi[0], hi[1], hi[2], hi[3], bb[0], bb[1]);
       mma_16816(o[d + 1], hi[0], hi[1], hi[2], hi[3], bb[2], bb[3]);
       mma_16816(o[d], lo[0], lo[1], lo[2], lo[3], bb[0], bb[1]);
