@@ -812,9 +812,10 @@ constexpr uint32_t kApDirectPairs = 64, kApDirectKeys = 192;  // rows x K/V head
 // 28.7 and 26.2, behind 2,048 (1,024) 34.3 and 36.3. 16 units of 8 x 32 heads behind 1,024: 84.8 and 57.8.
 constexpr int kApTcRowsFrom = 32, kApTcBlocks = 256, kApTcFewFrom = 16, kApTcFewBlocks = 1024;
 // Own entries of a row up to which single warps take them, where their warps (two per SM or more)
-// fill the SMs, and up to which they always do. 64 x 32 heads of up to 64, 128 and 256 entries: 14.1,
-// 20.6 and 35.8 us by warps, 22.0, 26.5 and 35.8 by tiles; 4 x 8 heads x 4 of up to 256: 11.2 and
-// 8.2; 32 x 8 heads x 4 of up to 64: 10.1 and 10.9.
+// fill the SMs, and up to which they always do. 64 x 32 heads of up to 64, 128 and 256 entries: 10.4,
+// 16.8 and 30.5 us by warps, 19.9, 23.6 and 31.6 by tiles; 4 x 8 heads x 4 of up to 256: 10.3 and
+// 6.1; behind a prefix of 256, 32 x 8 heads x 4 of up to 64: 10.5 and 11.3, 16 x 32: 9.4 and 11.1
+// (without one 32 x 8 x 4: 5.4 and 4.7).
 constexpr uint32_t kApWarpKeys = 256, kApWarpAlways = 64;
 
 int ap_wr(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
@@ -842,7 +843,7 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.tiles_o = (p.G + 16 * p.wr_o - 1) / (16 * p.wr_o);
   // Two rounds of three CTAs per SM at most; ranges long enough to pay for their start and their
   // record, shorter ones only where there are few CTAs (16 x 32 heads, prefix 1,000, own entries up
-  // to 128: 12.8 us with ranges of 256 and 128 keys at least, 15.7 with 128 and 64).
+  // to 128: 14.6 us with ranges of 256 and 128 keys at least, 16.0 with 128 and 64).
   const int want = 6 * num_sms();
   const auto ranges = [&](size_t ctas, uint32_t keys, int least) {
     const size_t s = (want + ctas - 1) / std::max<size_t>(ctas, 1);
@@ -852,9 +853,9 @@ ApPlan ap_plan(uint32_t M, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t num_
   p.S_p = 0;
   if (p.tc) {
     // One CTA per SM, and the own entries' CTAs run on the other SMs meanwhile: the cut whose
-    // estimated time is least, in us. A block takes ~1.5 (128 rows) or ~2.7 (256), a range's start
-    // and end ~5, and an SM gets through ~35 KB of own entries per us (they are taken to be half as
-    // long as they may be).
+    // estimated time is least, in us. A block is taken to cost 1.5 (128 rows; 1.4 alone) or 2.7 (256;
+    // 2.5 alone), a range's start and end 5, and an SM gets through ~35 KB of own entries per us (they
+    // are taken to be half as long as they may be).
     const double sms = num_sms(), blocks = (max_prefix + kApTcKeys - 1) / kApTcKeys;
     const double own = (double)M * nkv * max_own * 2.0 * hd / 35e3, block = p.tr_p > kApTcRows ? 2.7 : 1.5;
     double best = 0;

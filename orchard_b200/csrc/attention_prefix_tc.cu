@@ -2,14 +2,15 @@
 // many query rows: S = Q K^T and O += P V as tcgen05.mma with fp32 accumulators in tensor
 // memory, 128 query rows (rows x heads of one K/V head) by 128 keys at a time.
 //
-// Mathematics as in attention_prefix.cu. With 128 rows a block is 8.4 MFLOP against 64 KB of K
-// and V, past what mma.sync tiles sustain. Per block the products take ~1,050 cycles of the
-// tensor pipe and the 16,384 exponentials 1,024 cycles of the special-function units; two
-// groups of four warps keep both busy, one turning scores into weights while the tensor pipe
-// works for the other. A unit of up to 128 query rows gives the groups alternate blocks of keys;
-// with more (PAIR) a CTA takes 256 rows, a group 128 of them and every block: each block then
-// serves twice the rows, which halves the traffic from L2 (one tile of 128 rows per CTA was
-// bound by it: 4,000 cycles per block at 64 KB each).
+// Mathematics as in attention_prefix.cu. With 128 rows a block is 12.6 MFLOP (the scores, and V
+// with each of the weights' two terms) against 64 KB of K and V, past what mma.sync tiles sustain.
+// Per block the products take ~1,580 cycles of the tensor pipe (24 of 66) and the 16,384
+// exponentials 1,024 cycles of the special-function units; two groups of four warps keep both busy,
+// one turning scores into weights while the tensor pipe works for the other. A unit of up to 128
+// query rows gives the groups alternate blocks of keys; with more (PAIR) a CTA takes 256 rows, a
+// group 128 of them and every block: each block then serves twice the rows, which halves the
+// traffic from L2. 128 CTAs at once take 1.4 us per block with 128 rows, 2.5 with 256; head_dim 64
+// 1.3 and 2.1.
 //  * a producer thread brings K and V blocks by TMA (128-byte swizzle; K rows are the K-major
 //    operand of Q K^T, V rows the MN-major operand of P V), two slots each;
 //  * one warp issues the products, a lane elected at each;
