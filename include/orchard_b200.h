@@ -351,7 +351,8 @@ int orch_q4t_rms_qkv_rope_at(const void* tiled_qkv, const float* x, const float*
  * and position. K and V ([num_slots][num_kv_heads][max_seq][head_dim] fp16) change in place;
  * mass (fp32) and positions (int32), both [num_slots][num_kv_heads][max_seq], go to mass_out and
  * positions_out, which are the same buffers (in place) or both others (then only entries below
- * n of the rows' slots are written); lens_out[m] = n, in a buffer of its own. head_dim a multiple of 8;
+ * n of the rows' slots are written); lens_out[m] = n, in a buffer of its own (outputs that overlap
+ * anything otherwise than in place are refused). head_dim a multiple of 8;
  * max_seq at most 1,000,000. A row whose slot or length is out of range, or whose slot an
  * earlier row names, is left as it is and sets device check bit 8 (slot) / 2. */
 int orch_cache_evict(void* k_cache, void* v_cache, const float* mass, const int32_t* positions, const int32_t* lens,

@@ -461,6 +461,19 @@ extern "C" int orch_cache_evict(void* k_cache, void* v_cache, const float* mass,
                "cache_evict: mass and positions are both updated in place, or neither");
   if (max_seq > kEvMaxLen) return fail(ORCH_ERR_UNSUPPORTED, "cache_evict: max_seq above 1,000,000");
   if ((uint64_t)M * num_kv_heads > 0x7fffffffu) return fail(ORCH_ERR_UNSUPPORTED, "cache_evict: too many rows and heads");
+  // Outputs are in place or lie apart from everything that other CTAs may still read.
+  const size_t rows = (size_t)M * 4, entries = (size_t)num_slots * num_kv_heads * max_seq * 4;
+  const auto meet = [](const void* a, size_t an, const void* b, size_t bn) {
+    return a != nullptr && b != nullptr && (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+  };
+  const bool place = mass_out == mass;
+  ORCH_REQUIRE(!meet(lens_out, rows, lens, rows) && !meet(lens_out, rows, slots, rows) && !meet(lens_out, rows, mass, entries) &&
+                   !meet(lens_out, rows, positions, entries) && !meet(lens_out, rows, mass_out, entries) &&
+                   !meet(lens_out, rows, positions_out, entries) &&
+                   (place || (!meet(mass_out, entries, mass, entries) && !meet(positions_out, entries, positions, entries) &&
+                              !meet(mass_out, entries, positions_out, entries) && !meet(mass_out, entries, positions, entries) &&
+                              !meet(positions_out, entries, mass, entries))),
+               "cache_evict: outputs overlap inputs or each other");
   EvArgs a;
   a.kc = static_cast<__half*>(k_cache);
   a.vc = static_cast<__half*>(v_cache);
